@@ -313,7 +313,8 @@ def _own_norm(s):
 
 def _i8(s):
     x = s["x"].float()
-    scale = x.abs().amax(1) / 127
+    # the quotient rounded once (torch divides an fp32 tensor by a number as a product with its rounded reciprocal)
+    scale = (x.abs().amax(1).double() / 127).float()
     scale = torch.where(scale < torch.finfo(torch.float32).tiny, 0.0, scale)
     # to the nearest of the scale's multiples, in 64 bits: halves of the largest value lie next to a border
     codes = (x.double() / torch.where(scale > 0, scale, 1.0).double()[:, None]).round()
@@ -421,7 +422,7 @@ def exact(case, seed):
             branch = branch * s["gate"].double().repeat_interleave(case["gate_rows"] or case["rows"], 0)[:case["rows"]]
         y = s["x"].double() + case["scale"] * branch
         return {"y": y, "h": norm(y, s["pre_gamma"], s["pre_beta"]) if case["pre"] else torch.zeros_like(y)}
-    scale = s["x"].float().abs().max(1).values.div(127)  # the scale is kept in 32 bits: it is part of the definition
+    scale = s["x"].double().abs().max(1).values.div(127).float()  # kept in 32 bits: that is part of the definition
     scale[scale < 2.0 ** -126] = 0
     codes = torch.nan_to_num(torch.round(s["x"].double() / scale.double()[:, None]), nan=0.0)
     out = (codes @ s["w"].double().t()) * (scale.double()[:, None] * s["ws"].double()[None, :])
