@@ -425,6 +425,83 @@ int tk_merge_heads_f32(const float* ctx, int B, int S, int heads, int dh, float*
 int tk_tzgemm_batched(const void* A, const void* B, float* C, int M, int N, int K, int batch, long long stride_a,
                       long long stride_b, long long stride_c, float alpha, void* stream);
 
+/* ---- operators of a decoder block over packed tokens ----------------------------------------------------------
+ * (No counterpart in the reference.)  The pieces between the products of a transformer block that serves prompts of
+ * different lengths, packed row after row, and single tokens over a cache.  One call = one or two launches on `stream`;
+ * all buffers are device memory of the current device (a buffer of another one is refused with TK_ERR_ARGS), rows are
+ * `ld` elements apart, and everything works in a captured graph.  Calls with nothing to do (0 rows, tokens or
+ * sequences) return TK_OK.  Statistics, sums and scores are held in fp32 (8-bit products in 32-bit integers); a result
+ * is rounded once to its type.  Wide accesses need 16-byte aligned buffers and leading dimensions that are multiples of
+ * 8; other alignments take slower forms of the same operators where no refusal is stated. */
+typedef enum tk_type { TK_F32 = 0, TK_F16 = 1, TK_BF16 = 2 } tk_type;
+
+/* y = x + scale * gate * post(a), h = pre(y): the residual stream between two blocks in one pass.
+ *   a [rows][cols] of a_type; x, y of x_type; h of h_type.  x null: y = scale * gate * post(a); y or h null: not written;
+ *   y may be x.  post = 1: a is normalised first, with post_gamma / post_beta [cols] (null = 1 / 0); pre is the
+ *   norm of y (before y is rounded) that makes h, with pre_gamma / pre_beta.  layer 0: v / sqrt(mean v^2 + eps),
+ *   1: (v - mean) / sqrt(var + eps).  gate (null = 1): fp32, rows r share gate row r / gate_rows (gate_rows >= rows: one
+ *   row for all; 1: a row each; the tokens of a sequence each: a gate per sequence). */
+int tk_norm_residual_rows(const void* a, int a_type, long long ld_a, int post, const float* post_gamma,
+                          const float* post_beta, const float* gate, long long ld_gate, long long gate_rows, float scale,
+                          const void* x, long long ld_x, void* y, long long ld_y, int x_type, const float* pre_gamma,
+                          const float* pre_beta, void* h, long long ld_h, int h_type, int layer, float eps,
+                          long long rows, int cols, void* stream);
+
+/* Rows to 8-bit integers: scales[r] = max |x[r]| / 127, codes[r][c] = x[r][c] / scales[r] rounded to the nearest
+ * integer (the exact quotient with the fp32 scale; halves to even).  A row whose scale would be below 2^-126 gets scale 0
+ * and codes 0; a row with a NaN or an infinity gets a scale that is one and codes 0. */
+int tk_quantize_rows_i8(const void* x, int x_type, long long ld_x, void* codes, long long ld_codes, float* scales,
+                        long long rows, int cols, void* stream);
+
+/* out[m][n] = (sum_k A[m][k] B[n][k]) * scale_a[m] * scale_b[n] + bias[n]: 8-bit signed integers A [M][K] (tokens) and
+ * B [N][K] (output channels), exact 32-bit sums, fp32 scales [M] and [N], fp32 bias [N] or null, out [M][N] of out_type.
+ * Any M, N and K <= 131071 (TK_ERR_SHAPE beyond: the sums would overflow); A and B 16-byte aligned, lda and ldb multiples
+ * of 16 (TK_ERR_ALIGN). */
+int tk_i8gemm(const void* A, long long lda, const float* scale_a, const void* B, long long ldb, const float* scale_b,
+              const float* bias, void* out, long long ld_out, int out_type, int M, int N, int K, void* stream);
+
+/* The rotary plan of a model, host memory only: turns[i], i < rot_dim / 2 <= 256, full turns of pair i per position
+ * (base^(-2 i / rot_dim) / 2 pi before scaling), and the factor on cos and sin.
+ *   TK_ROPE_PLAIN   as trained
+ *   TK_ROPE_LINEAR  all pairs slower by `factor`
+ *   TK_ROPE_BASE    base * factor^(rot_dim / (rot_dim - 2)): the slowest pair is slower by `factor`, the fastest as trained
+ *   TK_ROPE_RAMP    pairs that turn more than `fast` times over trained_len as trained, those that turn less than `slow`
+ *                   times slower by `factor`, a linear mixture over the pairs between; magnitude 1 + 0.1 ln(factor) */
+enum { TK_ROPE_PLAIN = 0, TK_ROPE_LINEAR = 1, TK_ROPE_BASE = 2, TK_ROPE_RAMP = 3 };
+int tk_rope_turns(int rot_dim, double base, int scaling, double factor, double trained_len, double fast, double slow,
+                  double* turns, float* magnitude);
+
+/* The heads of three projections side by side, with rotary positions: x [tokens][ld_x], `heads` query heads of `dim`
+ * columns, then kv_heads key heads, then kv_heads value heads; bias (fp32, same columns, or null) is added first.  The
+ * first rot_dim elements of each query and key head are turned pair by pair, pair i by positions[t] * turns[i] turns
+ * (turns: device memory, binary64) and multiplied by `magnitude`; interleaved 1: pair i = elements 2 i and 2 i + 1,
+ * 0: elements i and i + rot_dim / 2.  q [tokens][heads][dim]; k and v [..][kv_heads][dim] go to row t, or with `slots`
+ * to row slots[t] of a cache of n_slots rows (a slot outside 0 .. n_slots - 1 is skipped: padding).  Two tokens must
+ * not share a slot.  dim <= 512.  Outputs must not overlap x. */
+int tk_rope_qkv(const void* x, int x_type, long long ld_x, const float* bias, const int* positions, const double* turns,
+                int rot_dim, int interleaved, float magnitude, long long tokens, int heads, int kv_heads, int dim, void* q,
+                long long ld_q, void* k, long long ld_k, void* v, long long ld_v, int out_type, const long long* slots,
+                long long n_slots, void* stream);
+
+/* softmax(scale q k^T) v over packed sequences.  Sequence i: query rows q_start[i] .. q_start[i + 1] - 1 of q
+ * [total_q][heads][dim] (ascending; rows before the first and behind the last sequence are left as they were), keys and
+ * values rows k_start[i] .. k_start[i] + k_len[i] - 1 of k and v [kv_rows][kv_heads][dim].  Query head h reads key head
+ * h / (heads / kv_heads).  causal: query t of q_len sees the keys j <= t + k_len - q_len.  A query that sees no key gives
+ * zeros and lse -infinity.  out like q; lse [total_q][heads] = log sum exp of the scaled scores, or null.  type TK_F16 or
+ * TK_BF16 for q, k, v and out; dim <= 256.  The three index arrays are device memory, read by the kernels (a captured
+ * graph replays with what they then hold); max_q and max_k, the longest q_len and k_len, choose the launch and may be
+ * larger than the truth.  Keys and values outside the sequences' rows are never used, whatever they hold; inside them a
+ * NaN or an infinity may reach every query of its sequence.
+ * workspace: device memory, 16-byte aligned, not shared by calls that may overlap; scratch for work split over long key
+ * axes.  A call splits as far as it has room; null or 0 bytes = no split.
+ * TK_ATTENTION_WORKSPACE bytes are enough for every split that pays. */
+#define TK_ATTENTION_WORKSPACE (64u << 20)
+int tk_attention_packed(const void* q, long long ld_q, const void* k, long long ld_k, const void* v, long long ld_v,
+                        void* out, long long ld_out, float* lse, int type, const int* q_start, const int* k_start,
+                        const int* k_len, int n_seqs, int total_q, int kv_rows, int max_q, int max_k, int heads,
+                        int kv_heads, int dim, float scale, int causal, void* workspace, size_t workspace_bytes,
+                        void* stream);
+
 /* ---- work-distribution plans (host only, no device needed) -------------------------------------------------
  * The enumeration code of the persistent kernels, run on the host so that its invariants can be checked
  * exhaustively (the reference relies on compute-sanitizer-free trial runs of generated binaries,

@@ -31,6 +31,18 @@ KEYS = ("gptb_tzgemm", "gptb_tzgemm_acc", "gptb_stencil", "gptb_cp", "gptb_mriq"
         "tzconv_sgemm", "tzconv_lbm", "tzconv_fft", "tzconv_cutcp")
 
 
+# C signatures of the entry points that take plain integers for addresses: p pointer, i int, l long long, z size_t,
+# f float.  Declared once, so that a call converts its arguments without building a ctypes object for each.
+_SIGNATURES = {
+    "tk_norm_residual_rows": "pilipp pll f pl pl i pp pl ii f l i p",
+    "tk_quantize_rows_i8": "pil pl p li p",
+    "tk_i8gemm": "pl p pl p p pl i iii p",
+    "tk_rope_qkv": "pil pp p ii f l iii pl pl pl i pl p",
+    "tk_attention_packed": "pl pl pl pl p i ppp iii ii iii f i pz p",
+}
+_CTYPE = {"p": C.c_void_p, "i": C.c_int, "l": C.c_longlong, "z": C.c_size_t, "f": C.c_float}
+
+
 class TackerError(RuntimeError):
     def __init__(self, status: int, where: str = ""):
         self.status = status
@@ -62,6 +74,8 @@ def lib() -> C.CDLL:
         l.tk_query.argtypes = [C.c_char_p, C.POINTER(KernelInfo)]
         l.tk_set_option.argtypes = [C.c_char_p, C.c_int]
         l.tk_get_option.argtypes = [C.c_char_p, C.POINTER(C.c_int)]
+        for name, signature in _SIGNATURES.items():
+            getattr(l, name).argtypes = [_CTYPE[c] for c in signature.replace(" ", "")]
         _lib = l
     return _lib
 

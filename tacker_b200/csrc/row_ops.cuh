@@ -1,0 +1,514 @@
+// Row kernels of a decoder block over packed tokens: element types chosen at run time, the residual stream between
+// two blocks (norm behind a block, gate, residual scale, norm before the next), rows rounded to 8-bit integers, and
+// the split of a fused projection into rotary query / key / value heads.
+// All of them are bound by memory traffic: every operand is read once and every result written once, 16 bytes per
+// access where the addresses allow it, with the row held in registers between the passes over it.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace tk {
+
+// element types of the C ABI (tk_type)
+constexpr int kF32 = 0, kF16 = 1, kBF16 = 2;
+
+__device__ __forceinline__ float load1(const void* p, int type, long long i) {
+    if (type == kF32) return static_cast<const float*>(p)[i];
+    if (type == kF16) return __half2float(static_cast<const __half*>(p)[i]);
+    return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
+}
+__device__ __forceinline__ void store1(void* p, int type, long long i, float v) {
+    if (type == kF32)
+        static_cast<float*>(p)[i] = v;
+    else if (type == kF16)
+        static_cast<__half*>(p)[i] = __float2half_rn(v);
+    else
+        static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
+}
+
+// eight consecutive elements as they lie in memory: 16 bytes of a 16-bit type, 32 bytes of fp32 (16-byte aligned)
+struct Raw8 {
+    uint4 lo, hi;
+};
+__device__ __forceinline__ Raw8 load_raw8(const void* p, int type, long long i) {
+    Raw8 r;
+    if (type == kF32) {
+        const uint4* s = reinterpret_cast<const uint4*>(static_cast<const float*>(p) + i);
+        r.lo = s[0];
+        r.hi = s[1];
+    } else {
+        r.lo = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + i);
+        r.hi = make_uint4(0u, 0u, 0u, 0u);
+    }
+    return r;
+}
+__device__ __forceinline__ void unpack2(uint32_t w, int type, float& a, float& b) {
+    if (type == kF16) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+        a = f.x, b = f.y;
+    } else {  // bf16 is the upper half of an fp32
+        a = __uint_as_float(w << 16), b = __uint_as_float(w & 0xffff0000u);
+    }
+}
+__device__ __forceinline__ void unpack8(const Raw8& r, int type, float (&v)[8]) {
+    if (type == kF32) {
+        v[0] = __uint_as_float(r.lo.x), v[1] = __uint_as_float(r.lo.y), v[2] = __uint_as_float(r.lo.z);
+        v[3] = __uint_as_float(r.lo.w), v[4] = __uint_as_float(r.hi.x), v[5] = __uint_as_float(r.hi.y);
+        v[6] = __uint_as_float(r.hi.z), v[7] = __uint_as_float(r.hi.w);
+    } else {
+        unpack2(r.lo.x, type, v[0], v[1]);
+        unpack2(r.lo.y, type, v[2], v[3]);
+        unpack2(r.lo.z, type, v[4], v[5]);
+        unpack2(r.lo.w, type, v[6], v[7]);
+    }
+}
+__device__ __forceinline__ uint32_t pack2(float a, float b, int type) {
+    if (type == kF16) {
+        const __half2 h = __floats2half2_rn(a, b);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ void store8(void* p, int type, long long i, const float (&v)[8]) {
+    if (type == kF32) {
+        float4* d = reinterpret_cast<float4*>(static_cast<float*>(p) + i);
+        d[0] = make_float4(v[0], v[1], v[2], v[3]);
+        d[1] = make_float4(v[4], v[5], v[6], v[7]);
+    } else {
+        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p) + i) = make_uint4(
+            pack2(v[0], v[1], type), pack2(v[2], v[3], type), pack2(v[4], v[5], type), pack2(v[6], v[7], type));
+    }
+}
+__device__ __forceinline__ void load8f(const float* p, int i, float (&v)[8]) {
+    const float4 a = __ldg(reinterpret_cast<const float4*>(p + i)), b = __ldg(reinterpret_cast<const float4*>(p + i) + 1);
+    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+}
+
+// Sum over the `tpr` threads of a row (a power of two, at least a warp); `slot` is a shared array of one float per warp
+// of the block.  Every thread of the block calls it, the same number of times.
+__device__ __forceinline__ float row_sum(float v, int tpr, float* slot) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    if (tpr == 32) return v;
+    const int warp = threadIdx.x >> 5, per = tpr >> 5, first = warp / per * per;
+    __syncthreads();  // the slots of the sum before have been read
+    if ((threadIdx.x & 31) == 0) slot[warp] = v;
+    __syncthreads();
+    // at most 32 warps share a row: one more butterfly over their partial sums, the same order in every warp
+    const int lane = threadIdx.x & 31;
+    float s = lane < per ? slot[first + lane] : 0.0f;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    return s;
+}
+
+// ---- the residual stream between two blocks ------------------------------------------------------------------------
+//   y = x + scale * gate * post(a),   h = pre(y)
+// post and pre are root-mean-square or layer norms over the row (or absent).  Statistics are fp32 sums of fp32 values;
+// the layer norm takes the mean first and the squares of the differences after it.  h is made from y before y is
+// rounded to its type: one rounding for each result.
+struct NormArgs {
+    const void* a;
+    const void* x;      // may be null (no residual stream) and may be y
+    void* y;            // may be null
+    void* h;            // may be null (no norm behind)
+    const float* post_gamma;
+    const float* post_beta;
+    const float* pre_gamma;
+    const float* pre_beta;
+    const float* gate;  // rows r of a share gate row r / gate_rows; null = 1
+    long long ld_a, ld_x, ld_y, ld_h, ld_gate, gate_rows, rows;
+    int a_type, x_type, h_type, cols, post, layer;
+    float scale, eps;
+};
+
+// One row per `tpr` threads, NV groups of eight columns per thread in registers.  x is fetched before the first sum so
+// that its latency and a's overlap.
+template <int NV>
+__global__ void norm_residual_kernel(const NormArgs p, const int tpr) {
+    __shared__ float slot[32];
+    const long long row = static_cast<long long>(blockIdx.x) * (blockDim.x / tpr) + threadIdx.x / tpr;
+    const int t = threadIdx.x & (tpr - 1);
+    const bool live = row < p.rows;
+    const float inv_cols = 1.0f / static_cast<float>(p.cols);
+    float v[NV][8];
+    Raw8 xr[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int c = (t + i * tpr) * 8;
+        if (live && c < p.cols) {
+            const Raw8 r = load_raw8(p.a, p.a_type, row * p.ld_a + c);
+            if (p.x) xr[i] = load_raw8(p.x, p.x_type, row * p.ld_x + c);
+            unpack8(r, p.a_type, v[i]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[i][j] = 0.0f;
+        }
+    }
+    // v <- (v - mean) * rstd over the columns of the row; the padding columns stay out of the sums
+    auto normalise = [&]() {
+        float mean = 0.0f;
+        if (p.layer) {
+            float s = 0.0f;
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) s += v[i][j];
+            mean = row_sum(s, tpr, slot) * inv_cols;
+        }
+        float q = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            if ((t + i * tpr) * 8 < p.cols) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    v[i][j] -= mean;
+                    q = fmaf(v[i][j], v[i][j], q);
+                }
+            }
+        }
+        const float rstd = rsqrtf(row_sum(q, tpr, slot) * inv_cols + p.eps);
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[i][j] *= rstd;
+    };
+    auto affine = [&](const float* gamma, const float* beta, int i, int c) {
+        if (gamma) {
+            float g[8];
+            load8f(gamma, c, g);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[i][j] *= g[j];
+        }
+        if (beta) {
+            float b[8];
+            load8f(beta, c, b);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[i][j] += b[j];
+        }
+    };
+    if (p.post) normalise();
+    const float* gate = p.gate && live ? p.gate + row / p.gate_rows * p.ld_gate : nullptr;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int c = (t + i * tpr) * 8;
+        if (!live || c >= p.cols) continue;
+        if (p.post) affine(p.post_gamma, p.post_beta, i, c);
+        if (gate) {
+            float g[8];
+            load8f(gate, c, g);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[i][j] *= g[j];
+        }
+        float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        if (p.x) unpack8(xr[i], p.x_type, x);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[i][j] = fmaf(p.scale, v[i][j], x[j]);
+        if (p.y) store8(p.y, p.x_type, row * p.ld_y + c, v[i]);
+    }
+    if (!p.h) return;
+    normalise();
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int c = (t + i * tpr) * 8;
+        if (!live || c >= p.cols) continue;
+        affine(p.pre_gamma, p.pre_beta, i, c);
+        store8(p.h, p.h_type, row * p.ld_h + c, v[i]);
+    }
+}
+
+// Any width, stride and alignment: one block per row, each pass reads the row again (from L2 after the first).  y is
+// written in the last pass only, so that it may be x.
+__global__ void norm_residual_any_kernel(const NormArgs p) {
+    __shared__ float slot[32];
+    const int tpr = blockDim.x;
+    const long long row = blockIdx.x;
+    const float inv_cols = 1.0f / static_cast<float>(p.cols);
+    const float* gate = p.gate ? p.gate + row / p.gate_rows * p.ld_gate : nullptr;
+    auto stats = [&](auto value, float& mean, float& rstd) {
+        mean = 0.0f;
+        if (p.layer) {
+            float s = 0.0f;
+            for (int c = threadIdx.x; c < p.cols; c += tpr) s += value(c);
+            mean = row_sum(s, tpr, slot) * inv_cols;
+        }
+        float q = 0.0f;
+        for (int c = threadIdx.x; c < p.cols; c += tpr) {
+            const float d = value(c) - mean;
+            q = fmaf(d, d, q);
+        }
+        rstd = rsqrtf(row_sum(q, tpr, slot) * inv_cols + p.eps);
+    };
+    float m1 = 0.0f, r1 = 1.0f, m2 = 0.0f, r2 = 1.0f;
+    if (p.post) stats([&](int c) { return load1(p.a, p.a_type, row * p.ld_a + c); }, m1, r1);
+    auto stream = [&](int c) {
+        float v = load1(p.a, p.a_type, row * p.ld_a + c);
+        if (p.post) {
+            v = (v - m1) * r1;
+            if (p.post_gamma) v *= p.post_gamma[c];
+            if (p.post_beta) v += p.post_beta[c];
+        }
+        if (gate) v *= gate[c];
+        return fmaf(p.scale, v, p.x ? load1(p.x, p.x_type, row * p.ld_x + c) : 0.0f);
+    };
+    if (p.h) stats(stream, m2, r2);
+    for (int c = threadIdx.x; c < p.cols; c += tpr) {
+        const float y = stream(c);
+        if (p.y) store1(p.y, p.x_type, row * p.ld_y + c, y);
+        if (p.h) {
+            float h = (y - m2) * r2;
+            if (p.pre_gamma) h *= p.pre_gamma[c];
+            if (p.pre_beta) h += p.pre_beta[c];
+            store1(p.h, p.h_type, row * p.ld_h + c, h);
+        }
+    }
+}
+
+// ---- rows to 8-bit integers ----------------------------------------------------------------------------------------
+//   scale_r = max_c |x_rc| / 127 (fp32),   code_rc = x_rc / scale_r rounded to the nearest integer, halves to even
+// The rounding is that of the exact quotient: an fp32 quotient can be rounded onto a half that the exact one misses (the
+// half of the largest value is such a place), so the candidate is put right by the remainder x - k s, which one fma
+// gives without rounding: it is a multiple of the last place of s (or of x) below 2^24 such places.
+// Rows whose scale is no normal number (all zero, or below 127 * 2^-126) get scale 0 and codes 0; a row with a NaN or an
+// infinity gets that as its scale and codes 0, so that products with it are NaN.
+__device__ __forceinline__ float row_scale(uint32_t amax_bits) {
+    const float amax = __uint_as_float(amax_bits);
+    if (amax_bits >= 0x7f800000u) return amax;
+    const float s = __fdiv_rn(amax, 127.0f);
+    return s < 1.17549435e-38f ? 0.0f : s;
+}
+__device__ __forceinline__ int row_code(float x, float s, float inv) {
+    float k = rintf(x * inv);
+    const float r2 = 2.0f * fmaf(-k, s, x);
+    const bool odd = (static_cast<int>(k) & 1) != 0;
+    if (r2 > s || (r2 == s && odd)) k += 1.0f;
+    if (r2 < -s || (r2 == -s && odd)) k -= 1.0f;
+    return static_cast<int>(fminf(fmaxf(k, -127.0f), 127.0f));
+}
+// |x| as its bits: as unsigned numbers they are ordered like the values, with NaN above everything
+__device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+__device__ __forceinline__ uint32_t row_umax(uint32_t v, int tpr, uint32_t* slot) {
+    v = __reduce_max_sync(0xffffffffu, v);
+    if (tpr == 32) return v;
+    const int warp = threadIdx.x >> 5, per = tpr >> 5, first = warp / per * per, lane = threadIdx.x & 31;
+    if (lane == 0) slot[warp] = v;
+    __syncthreads();
+    return __reduce_max_sync(0xffffffffu, lane < per ? slot[first + lane] : 0u);
+}
+
+struct QuantArgs {
+    const void* x;
+    int8_t* codes;
+    float* scales;
+    long long ld_x, ld_codes, rows;
+    int type, cols;
+};
+
+template <int NV>
+__global__ void quantize_rows_kernel(const QuantArgs p, const int tpr) {
+    __shared__ uint32_t slot[32];
+    const long long row = static_cast<long long>(blockIdx.x) * (blockDim.x / tpr) + threadIdx.x / tpr;
+    const int t = threadIdx.x & (tpr - 1);
+    const bool live = row < p.rows;
+    float v[NV][8];
+    uint32_t m = 0u;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int c = (t + i * tpr) * 8;
+        if (live && c < p.cols) {
+            unpack8(load_raw8(p.x, p.type, row * p.ld_x + c), p.type, v[i]);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) m = max(m, abs_bits(v[i][j]));
+        }
+    }
+    m = row_umax(m, tpr, slot);
+    if (!live) return;
+    const float s = row_scale(m);
+    const bool usable = s > 0.0f && m < 0x7f800000u;
+    const float inv = usable ? 1.0f / s : 0.0f;
+    if (t == 0) p.scales[row] = s;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int c = (t + i * tpr) * 8;
+        if (c >= p.cols) continue;
+        uint32_t w[2] = {0u, 0u};
+        if (usable) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                w[j >> 2] |= (static_cast<uint32_t>(row_code(v[i][j], s, inv)) & 0xffu) << (8 * (j & 3));
+        }
+        *reinterpret_cast<uint2*>(p.codes + row * p.ld_codes + c) = make_uint2(w[0], w[1]);
+    }
+}
+
+__global__ void quantize_rows_any_kernel(const QuantArgs p) {
+    __shared__ uint32_t slot[32];
+    const long long row = blockIdx.x;
+    uint32_t m = 0u;
+    for (int c = threadIdx.x; c < p.cols; c += blockDim.x) m = max(m, abs_bits(load1(p.x, p.type, row * p.ld_x + c)));
+    m = row_umax(m, blockDim.x, slot);
+    const float s = row_scale(m);
+    const bool usable = s > 0.0f && m < 0x7f800000u;
+    const float inv = usable ? 1.0f / s : 0.0f;
+    if (threadIdx.x == 0) p.scales[row] = s;
+    for (int c = threadIdx.x; c < p.cols; c += blockDim.x)
+        p.codes[row * p.ld_codes + c] =
+            usable ? static_cast<int8_t>(row_code(load1(p.x, p.type, row * p.ld_x + c), s, inv)) : static_cast<int8_t>(0);
+}
+
+// ---- rotary head split ---------------------------------------------------------------------------------------------
+// One token per block.  Row t of x holds heads query heads, kv_heads key heads and kv_heads value heads side by side;
+// pair i of a query or key head is turned by 2 pi pos_t turns_i.  The product is taken in binary64 and reduced to a
+// fraction of a turn there: an fp32 angle at position 10^6 is off by 0.06.  What is left in [-1/2, 1/2] loses nothing
+// in fp32.  The angles of a token serve all its heads and are computed once, into shared memory.
+struct RopeArgs {
+    const void* x;
+    const float* bias;          // [(heads + 2 kv_heads) dim] or null
+    const int* pos;
+    const double* turns;        // [rot / 2]
+    const long long* slots;     // row of k and v for each token (negative or >= n_slots: none), or null = the token
+    void* q;
+    void* k;
+    void* v;
+    long long ld_x, ld_q, ld_k, ld_v, n_slots;
+    int x_type, out_type, heads, kv_heads, dim, rot, interleaved;
+    float magnitude;
+};
+constexpr int kRopeMaxDim = 512;
+
+__device__ __forceinline__ void rope_angles(const RopeArgs& p, long long token, float2* cs) {
+    for (int i = threadIdx.x; i < p.rot / 2; i += blockDim.x) {
+        double a = static_cast<double>(p.pos[token]) * p.turns[i];
+        a -= rint(a);
+        float s, c;
+        sincospif(2.0f * static_cast<float>(a), &s, &c);
+        cs[i] = make_float2(c * p.magnitude, s * p.magnitude);
+    }
+}
+
+// where head `head` of the row goes: q, or the slot's row of k or v; null = nowhere
+__device__ __forceinline__ void* rope_dest(const RopeArgs& p, long long token, long long slot, int head, long long& at) {
+    if (head < p.heads) {
+        at = token * p.ld_q + static_cast<long long>(head) * p.dim;
+        return p.q;
+    }
+    if (slot < 0) return nullptr;
+    head -= p.heads;
+    if (head < p.kv_heads) {
+        at = slot * p.ld_k + static_cast<long long>(head) * p.dim;
+        return p.k;
+    }
+    at = slot * p.ld_v + static_cast<long long>(head - p.kv_heads) * p.dim;
+    return p.v;
+}
+__device__ __forceinline__ long long rope_slot(const RopeArgs& p, long long token) {
+    if (!p.slots) return token;
+    const long long s = p.slots[token];
+    return s < p.n_slots ? s : -1;
+}
+
+__global__ void rope_qkv_any_kernel(const RopeArgs p) {
+    __shared__ float2 cs[kRopeMaxDim / 2];
+    const long long token = blockIdx.x;
+    rope_angles(p, token, cs);
+    __syncthreads();
+    const long long slot = rope_slot(p, token);
+    const int total = (p.heads + 2 * p.kv_heads) * p.dim;
+    auto value = [&](int e) { return load1(p.x, p.x_type, token * p.ld_x + e) + (p.bias ? p.bias[e] : 0.0f); };
+    for (int e = threadIdx.x; e < total; e += blockDim.x) {
+        const int head = e / p.dim, d = e - head * p.dim;
+        long long at;
+        void* dst = rope_dest(p, token, slot, head, at);
+        if (!dst) continue;
+        float o = value(e);
+        if (head < p.heads + p.kv_heads && d < p.rot) {
+            const int half = p.rot / 2;
+            const int pair = p.interleaved ? d >> 1 : (d < half ? d : d - half);
+            const bool second = p.interleaved ? (d & 1) != 0 : d >= half;
+            const int apart = p.interleaved ? 1 : half;
+            const float other = value(second ? e - apart : e + apart);
+            const float2 w = cs[pair];
+            o = second ? o * w.x + other * w.y : o * w.x - other * w.y;
+        }
+        store1(dst, p.out_type, at + d, o);
+    }
+}
+
+// The same, sixteen elements per step: the two groups of eight whose pairs lie half the rotary part apart, or sixteen
+// neighbours (pairs side by side, elements behind the rotary part, values).  dim and rot are multiples of 16.  The
+// first step's loads are issued before the angles are computed.
+__global__ void rope_qkv_vec_kernel(const RopeArgs p) {
+    __shared__ float2 cs[kRopeMaxDim / 2];
+    const long long token = blockIdx.x;
+    const int per = p.dim / 16, nrot = p.rot / 16, units = (p.heads + 2 * p.kv_heads) * per;
+    auto place = [&](int u, int& head, int& d0, int& d1) {
+        head = u / per;
+        const int c = u - head * per;
+        const bool apart = !p.interleaved && c < nrot && head < p.heads + p.kv_heads;
+        d0 = apart ? 8 * c : 16 * c;
+        d1 = apart ? p.rot / 2 + 8 * c : 16 * c + 8;
+        return c;
+    };
+    int u = threadIdx.x, head = 0, d0 = 0, d1 = 0, c = 0;
+    Raw8 r0, r1;
+    if (u < units) {
+        c = place(u, head, d0, d1);
+        r0 = load_raw8(p.x, p.x_type, token * p.ld_x + head * p.dim + d0);
+        r1 = load_raw8(p.x, p.x_type, token * p.ld_x + head * p.dim + d1);
+    }
+    const long long slot = rope_slot(p, token);
+    rope_angles(p, token, cs);
+    __syncthreads();
+    while (u < units) {
+        float a[8], b[8];
+        unpack8(r0, p.x_type, a);
+        unpack8(r1, p.x_type, b);
+        const int head_now = head, d0_now = d0, d1_now = d1, c_now = c;
+        u += blockDim.x;
+        if (u < units) {
+            c = place(u, head, d0, d1);
+            r0 = load_raw8(p.x, p.x_type, token * p.ld_x + head * p.dim + d0);
+            r1 = load_raw8(p.x, p.x_type, token * p.ld_x + head * p.dim + d1);
+        }
+        long long at;
+        void* dst = rope_dest(p, token, slot, head_now, at);
+        if (!dst) continue;
+        if (p.bias) {
+            float w[8];
+            load8f(p.bias, head_now * p.dim + d0_now, w);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) a[j] += w[j];
+            load8f(p.bias, head_now * p.dim + d1_now, w);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) b[j] += w[j];
+        }
+        if (head_now < p.heads + p.kv_heads && c_now < nrot) {
+            if (p.interleaved) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float2 wa = cs[8 * c_now + j], wb = cs[8 * c_now + 4 + j];
+                    const float a0 = a[2 * j], a1 = a[2 * j + 1], b0 = b[2 * j], b1 = b[2 * j + 1];
+                    a[2 * j] = a0 * wa.x - a1 * wa.y;
+                    a[2 * j + 1] = a1 * wa.x + a0 * wa.y;
+                    b[2 * j] = b0 * wb.x - b1 * wb.y;
+                    b[2 * j + 1] = b1 * wb.x + b0 * wb.y;
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const float2 w = cs[8 * c_now + j];
+                    const float a0 = a[j];
+                    a[j] = a0 * w.x - b[j] * w.y;
+                    b[j] = b[j] * w.x + a0 * w.y;
+                }
+            }
+        }
+        store8(dst, p.out_type, at + d0_now, a);
+        store8(dst, p.out_type, at + d1_now, b);
+    }
+}
+
+}  // namespace tk

@@ -1,4 +1,7 @@
 // libtacker_b200.so: the C-ABI entry points (see include/tacker_b200.h for the contract).
+#include <cmath>
+#include <initializer_list>
+
 #include "host_launch.cuh"
 #include "more_kernels.cuh"
 
@@ -1585,6 +1588,11 @@ TK_API int tk_tzgemm_batched(const void* A, const void* B, float* C, int M, int 
     if (rc != TK_OK) return rc;
     return run_tzgemm(c, static_cast<unsigned>(d->sm_count), static_cast<cudaStream_t>(stream));
 }
+
+// =================================================================================================
+// operators of a decoder block over packed tokens
+// =================================================================================================
+#include "decoder_entries.cuh"
 
 // =================================================================================================
 // work-distribution plans, evaluated on the host (no device needed): the same enumeration code the

@@ -541,4 +541,52 @@ def tzgemm_batched(A, B, Cm, M, N, K, batch, alpha=1.0, stride_a=0, stride_b=0, 
           "tk_tzgemm_batched")
 
 
+# ---- operators of a decoder block over packed tokens ----------------------------------------------------------
+F32, F16, BF16 = 0, 1, 2
+ROPE_PLAIN, ROPE_LINEAR, ROPE_BASE, ROPE_RAMP = 0, 1, 2, 3
+ATTENTION_WORKSPACE = 64 << 20
+
+
+def norm_residual_rows(a, a_type, ld_a, post, post_gamma, post_beta, gate, ld_gate, gate_rows, scale, x, ld_x, y, ld_y,
+                       x_type, pre_gamma, pre_beta, h, ld_h, h_type, layer, eps, rows, cols, stream: int = 0) -> None:
+    """y = x + scale * gate * post(a), h = pre(y): root-mean-square (layer 0) or layer norms behind and before a block."""
+    check(lib().tk_norm_residual_rows(a, a_type, ld_a, post, post_gamma, post_beta, gate, ld_gate, gate_rows, scale, x,
+                                      ld_x, y, ld_y, x_type, pre_gamma, pre_beta, h, ld_h, h_type, layer, eps, rows, cols,
+                                      stream), "tk_norm_residual_rows")
+
+
+def quantize_rows_i8(x, x_type, ld_x, codes, ld_codes, scales, rows, cols, stream: int = 0) -> None:
+    """Rows to 8-bit integers with a scale each (max |row| / 127)."""
+    check(lib().tk_quantize_rows_i8(x, x_type, ld_x, codes, ld_codes, scales, rows, cols, stream), "tk_quantize_rows_i8")
+
+
+def i8gemm(A, lda, scale_a, B, ldb, scale_b, bias, out, ld_out, out_type, M, N, K, stream: int = 0) -> None:
+    """out = (A B^T) * scale_a[m] * scale_b[n] + bias[n] of 8-bit integers."""
+    check(lib().tk_i8gemm(A, lda, scale_a, B, ldb, scale_b, bias, out, ld_out, out_type, M, N, K, stream), "tk_i8gemm")
+
+
+def rope_turns(rot_dim, base=10000.0, scaling=ROPE_PLAIN, factor=1.0, trained_len=0.0, fast=32.0, slow=1.0):
+    """The rotary plan of a model: (turns of each pair per position, factor on cos and sin)."""
+    turns, magnitude = (C.c_double * max(1, rot_dim // 2))(), C.c_float(0.0)
+    check(lib().tk_rope_turns(rot_dim, C.c_double(base), scaling, C.c_double(factor), C.c_double(trained_len),
+                              C.c_double(fast), C.c_double(slow), turns, C.byref(magnitude)), "tk_rope_turns")
+    return list(turns), magnitude.value
+
+
+def rope_qkv(x, x_type, ld_x, bias, positions, turns, rot_dim, interleaved, magnitude, tokens, heads, kv_heads, dim, q, ld_q,
+             k, ld_k, v, ld_v, out_type, slots=0, n_slots=0, stream: int = 0) -> None:
+    """Fused projections -> query, key and value heads with rotary positions, keys and values into a cache's slots."""
+    check(lib().tk_rope_qkv(x, x_type, ld_x, bias, positions, turns, rot_dim, interleaved, magnitude, tokens, heads, kv_heads,
+                            dim, q, ld_q, k, ld_k, v, ld_v, out_type, slots, n_slots, stream), "tk_rope_qkv")
+
+
+def attention_packed(q, ld_q, k, ld_k, v, ld_v, out, ld_out, lse, type, q_start, k_start, k_len, n_seqs, total_q, kv_rows,
+                     max_q, max_k, heads, kv_heads, dim, scale, causal, workspace=0, workspace_bytes=0,
+                     stream: int = 0) -> None:
+    """softmax(scale q k^T) v over packed sequences: prompts, chunks behind a cache, single tokens."""
+    check(lib().tk_attention_packed(q, ld_q, k, ld_k, v, ld_v, out, ld_out, lse, type, q_start, k_start, k_len, n_seqs,
+                                    total_q, kv_rows, max_q, max_k, heads, kv_heads, dim, scale, causal, workspace,
+                                    workspace_bytes, stream), "tk_attention_packed")
+
+
 __all__ = [n for n in dir() if not n.startswith("_")]
