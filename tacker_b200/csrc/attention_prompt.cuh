@@ -1,0 +1,502 @@
+// Attention over packed sequences on the tensor cores: prompts and chunks of prompts (the definition is in
+// attention_rows.cuh).
+//
+// Rows.  The query heads that share a key head are rows of one tile: a tile has 128 / group tokens x group heads, token
+// after token, so that a key tile fetched once serves the whole group and short sequences still fill rows.  One work item
+// is two tiles (256 rows) of one sequence and key head; one persistent CTA per SM walks the items.
+//
+//   warps 0..3, 4..7  softmax of tile 0 and of tile 1, one row per thread; at the end of an item they write its rows
+//   warp 8            issues the MMAs of both tiles:  S = Q K^T (128 x 128, fp32, TMEM),  O += P V  with P read from TMEM
+//   warp 9            TMA: Q tiles, then K and V tiles of 128 keys through a ring
+//
+// While the softmax of one tile runs, the tensor cores work for the other one.  P overwrites the columns of its S.
+// The running maximum is raised (and O multiplied by what that costs, in TMEM) only when the new one exceeds it by more
+// than 2^8: weights stay below 2^8, well inside the 16-bit types, the sums are fp32, and the final division makes it
+// exact; after the first tiles almost no item pays for a rescale.  P is rounded to the type of V because the tensor
+// cores take two operands of one type; the row sum is taken before that rounding.
+//
+// Masks.  Keys beyond a row's limit get -infinity whatever their score is.  Weights of hidden keys are exact zeros, and
+// the values behind the sequence's last key within the last 16 that an MMA reads are zeroed in shared memory, so that
+// nothing they hold (NaN included) can enter.
+//
+// Bound: per key tile and SM the two tiles take 2 x 2 x 512 cycles of the tensor pipe (head size 128) and 32768 powers of
+// two = 2048 cycles of the special-function units; both run at the same time.
+#pragma once
+#include <cuda.h>
+
+#include "attention_rows.cuh"
+#include "gemm_role2.cuh"
+
+namespace tk {
+
+// D[tmem] (+)= A[tmem] * B[smem]: the weights come from tensor memory
+__device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
+                                            uint32_t accumulate) {
+    asm volatile(
+        "{\n"
+        ".reg .pred p;\n"
+        "setp.ne.b32 p, %4, 0;\n"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n"
+        "}\n" ::"r"(d_tmem),
+        "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+__device__ __forceinline__ void tmem_st_32x32(uint32_t taddr, const uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+        "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+        "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+        "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// V as the B operand of P V: its rows are keys (the k of the product), 64 head elements = 128 bytes contiguous, written
+// by TMA with the 128-byte swizzle.  The operand is therefore "MN-major": eight keys apart is the stride byte offset,
+// 64 head elements apart (the next box) the leading byte offset.
+__device__ __forceinline__ uint64_t umma_smem_desc_sw128_mn(uint32_t smem_addr, uint32_t box_bytes) {
+    uint64_t d = 0;
+    d |= static_cast<uint64_t>((smem_addr & 0x3FFFFu) >> 4);
+    d |= static_cast<uint64_t>(box_bytes >> 4) << 16;
+    d |= static_cast<uint64_t>(1024u >> 4) << 32;
+    d |= 1ull << 46;
+    d |= 2ull << 61;
+    return d;
+}
+
+constexpr int kAttnThreads = 320;
+constexpr int kAttnKeys = 128;  // keys of a tile
+
+template <int D>
+struct AttnSmem {
+    static constexpr int kBoxBytes = 128 * 128;  // 128 rows x 64 elements
+    static constexpr int kTileBytes = (D / 64) * kBoxBytes;
+    static constexpr int kStages = D == 128 ? 5 : 10;
+    static constexpr int kKvOffset = 2 * kTileBytes;
+    static constexpr int kBarOffset = kKvOffset + kStages * kTileBytes;
+    // barriers: ring full / empty, Q full / empty per tile, S full, P full, O full per tile
+    static constexpr int kNumBars = 2 * kStages + 10;
+    static constexpr int kTmemSlotOffset = kBarOffset + kNumBars * 8;
+    static constexpr int kAbortOffset = kTmemSlotOffset + 4;
+    static constexpr int kBytes = kAbortOffset + 4;
+};
+
+// One work item: two tiles of query rows of one sequence and key head.
+struct AttnItem {
+    AttnSeq s;
+    int kv;    // key head
+    int t0;    // first token of tile 0
+    int n[2];  // key tiles that some row of the tile sees
+};
+
+// Finds work items by index, in ascending order of calls.  Items of a sequence run from its last tokens (which see the
+// most keys) to its first, key heads innermost.  All lanes of a warp call it together.
+struct AttnWalk {
+    int base;         // first sequence of the window of 32 that the search stands at
+    long long before; // items of the sequences before it
+    __device__ __forceinline__ void init() { base = 0, before = 0; }
+
+    __device__ __forceinline__ bool find(const AttnArgs& p, long long index, int tile_tokens, int lane, AttnItem& it) {
+        const int pair_tokens = 2 * tile_tokens;
+        while (base < p.n_seqs) {
+            AttnSeq s;
+            s.q_len = 0, s.q0 = 0, s.k0 = 0, s.k_len = 0;
+            if (base + lane < p.n_seqs) s.load(p, base + lane);
+            const long long mine = static_cast<long long>((s.q_len + pair_tokens - 1) / pair_tokens) * p.kv_heads;
+            long long upto = mine;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const long long u = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= o) upto += u;
+            }
+            const uint32_t hit = __ballot_sync(0xffffffffu, before + upto > index);
+            if (hit) {
+                const int l = __ffs(hit) - 1;
+                it.s.q0 = __shfl_sync(0xffffffffu, s.q0, l);
+                it.s.q_len = __shfl_sync(0xffffffffu, s.q_len, l);
+                it.s.k0 = __shfl_sync(0xffffffffu, s.k0, l);
+                it.s.k_len = __shfl_sync(0xffffffffu, s.k_len, l);
+                const long long of = __shfl_sync(0xffffffffu, mine, l);
+                const long long at = index - before - (__shfl_sync(0xffffffffu, upto, l) - of);
+                it.kv = static_cast<int>(at % p.kv_heads);
+                it.t0 = static_cast<int>((of - 1 - at) / p.kv_heads) * pair_tokens;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int first = it.t0 + h * tile_tokens;
+                    const int last = min(first + tile_tokens, it.s.q_len) - 1;
+                    int keys = it.s.k_len;
+                    if (p.causal) keys = min(keys, max(0, last + 1 + it.s.k_len - it.s.q_len));
+                    it.n[h] = last < first ? 0 : (keys + kAttnKeys - 1) / kAttnKeys;
+                }
+                return true;
+            }
+            before += __shfl_sync(0xffffffffu, upto, 31);
+            base += 32;
+        }
+        return false;
+    }
+};
+
+// item of CTA c in round r: every other round runs backwards, so that long and short items even out
+__device__ __forceinline__ long long attn_index(int round) {
+    const long long g = gridDim.x;
+    return round * g + ((round & 1) ? g - 1 - blockIdx.x : static_cast<long long>(blockIdx.x));
+}
+
+template <int D, int TYPE>
+__global__ void __launch_bounds__(kAttnThreads, 1)
+attention_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
+                        const __grid_constant__ CUtensorMap tmap_v, const AttnArgs p, const int group,
+                        unsigned* status) {
+    using L = AttnSmem<D>;
+    constexpr int ST = L::kStages;
+    constexpr uint32_t kO = 256;  // TMEM: S / P of tile 0 at column 0, of tile 1 at 128, O of the tiles at 256 and 384
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = align_smem_1024(smem_raw);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t base = smem_u32(smem);
+    const uint32_t bars = base + L::kBarOffset;
+    auto kv_full = [&](int s) { return bars + 8u * s; };
+    auto kv_empty = [&](int s) { return bars + 8u * (ST + s); };
+    auto q_full = [&](int h) { return bars + 8u * (2 * ST + h); };
+    auto q_empty = [&](int h) { return bars + 8u * (2 * ST + 2 + h); };
+    auto s_full = [&](int h) { return bars + 8u * (2 * ST + 4 + h); };
+    auto p_full = [&](int h) { return bars + 8u * (2 * ST + 6 + h); };
+    auto o_full = [&](int h) { return bars + 8u * (2 * ST + 8 + h); };
+    volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + L::kTmemSlotOffset);
+    volatile uint32_t* abort_flag = reinterpret_cast<volatile uint32_t*>(smem + L::kAbortOffset);
+
+    if (warp == 8) {
+        if (lane == 0) {
+            *abort_flag = 0u;
+            for (int s = 0; s < ST; ++s) {
+                mbar_init(kv_full(s), 1);
+                mbar_init(kv_empty(s), 1);
+            }
+            for (int h = 0; h < 2; ++h) {
+                mbar_init(q_full(h), 1);
+                mbar_init(q_empty(h), 1);
+                mbar_init(s_full(h), 1);
+                mbar_init(p_full(h), 4);  // one arrival per softmax warp
+                mbar_init(o_full(h), 1);
+            }
+            fence_mbar_init();
+        }
+        __syncwarp();
+        tmem_alloc(smem_u32(const_cast<uint32_t*>(tmem_slot)), 512);
+        tmem_relinquish();
+    }
+    if (warp == 9 && lane == 0) {
+        tma_prefetch_desc(&tmap_q);
+        tma_prefetch_desc(&tmap_k);
+        tma_prefetch_desc(&tmap_v);
+    }
+    tc_fence_before_sync();
+    __syncthreads();
+    tc_fence_after_sync();
+    const uint32_t tmem = *tmem_slot;
+    const int tile_tokens = 128 / group;
+
+    AttnWalk walk;
+    walk.init();
+    AttnItem it;
+    // a wait of a whole warp: one verdict for all lanes
+    auto wait = [&](uint32_t bar, uint32_t parity, unsigned code) {
+        return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, status, code)) != 0;
+    };
+
+    if (warp == 9) {
+        // ---------------- TMA producer ----------------
+        int stage = 0;
+        uint32_t phase = 0, q_phase[2] = {0, 0};
+        bool ok = true;
+        const uint32_t q_bytes = static_cast<uint32_t>((D / 64) * tile_tokens * group * 128);
+        for (int round = 0; ok && walk.find(p, attn_index(round), tile_tokens, lane, it); ++round) {
+            if (lane == 0) {
+                const int n = max(it.n[0], it.n[1]);
+                auto load_q = [&](int h) {
+                    if (it.n[h] == 0) return true;
+                    if (!mbar_wait(q_empty(h), q_phase[h] ^ 1u, abort_flag, status, DEV_TIMEOUT_EMPTY)) return false;
+                    q_phase[h] ^= 1u;
+                    mbar_arrive_expect_tx(q_full(h), q_bytes);
+#pragma unroll
+                    for (int x = 0; x < D; x += 64)
+                        tma_load_tile(base + h * L::kTileBytes + (x / 64) * L::kBoxBytes, &tmap_q, q_full(h), x,
+                                      it.kv * group, it.s.q0 + it.t0 + h * tile_tokens);
+                    return true;
+                };
+                auto load_kv = [&](const CUtensorMap* map, int j) {
+                    if (!mbar_wait(kv_empty(stage), phase ^ 1u, abort_flag, status, DEV_TIMEOUT_EMPTY)) return false;
+                    mbar_arrive_expect_tx(kv_full(stage), L::kTileBytes);
+#pragma unroll
+                    for (int x = 0; x < D; x += 64)
+                        tma_load_tile(base + L::kKvOffset + stage * L::kTileBytes + (x / 64) * L::kBoxBytes, map,
+                                      kv_full(stage), x, it.kv, it.s.k0 + j * kAttnKeys);
+                    if (++stage == ST) {
+                        stage = 0;
+                        phase ^= 1u;
+                    }
+                    return true;
+                };
+                ok = load_q(0);
+                for (int j = 0; ok && j < n; ++j) {
+                    ok = load_kv(&tmap_k, j);
+                    if (ok && j == 0) ok = load_q(1);
+                    ok = ok && load_kv(&tmap_v, j);
+                }
+            }
+            ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+        }
+        // the last commits arrive on the empty barriers asynchronously: the CTA must not retire before they have landed
+        if (lane == 0) {
+            for (int s = 0; s < ST && ok; ++s) {
+                ok = mbar_wait(kv_empty(stage), phase ^ 1u, abort_flag, status, DEV_TIMEOUT_EMPTY);
+                if (++stage == ST) {
+                    stage = 0;
+                    phase ^= 1u;
+                }
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                ok = ok && mbar_wait(q_empty(h), q_phase[h] ^ 1u, abort_flag, status, DEV_TIMEOUT_EMPTY);
+        }
+    } else if (warp == 8) {
+        // ---------------- MMA issuer ----------------
+        const uint32_t fmt = TYPE == kBF16 ? (1u << 7) | (1u << 10) : 0u;  // A and B format: 0 = fp16, 1 = bf16
+        const uint32_t idesc_s = umma_idesc_f16_f32(128, kAttnKeys) | fmt;
+        const uint32_t idesc_o = umma_idesc_f16_f32(128, D) | fmt | (1u << 16);  // B = V is MN-major
+        int stage = 0;  // ring position: K_0 V_0 K_1 V_1 ... of one item after another
+        uint32_t phase = 0, q_phase[2] = {0, 0}, p_phase[2] = {0, 0};
+        bool ok = true;
+        auto advance = [&](int& st, uint32_t& ph) {
+            if (++st == ST) {
+                st = 0;
+                ph ^= 1u;
+            }
+        };
+        auto scores = [&](int h, int st) {
+            if (lane == 0) {
+                const uint32_t q = base + h * L::kTileBytes, k = base + L::kKvOffset + st * L::kTileBytes;
+#pragma unroll
+                for (int x = 0; x < D / 16; ++x) {
+                    const uint32_t off = (x >> 2) * L::kBoxBytes;
+                    umma_f16(tmem + h * 128, umma_smem_desc_sw128(q + off) + 2u * (x & 3),
+                             umma_smem_desc_sw128(k + off) + 2u * (x & 3), idesc_s, x != 0);
+                }
+                umma_commit(s_full(h));
+            }
+        };
+        for (int round = 0; ok && walk.find(p, attn_index(round), tile_tokens, lane, it); ++round) {
+            const int n = max(it.n[0], it.n[1]);
+            if (n == 0) continue;
+            // the first scores of both tiles
+            ok = wait(kv_full(stage), phase, DEV_TIMEOUT_FULL);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                if (!ok || it.n[h] == 0) continue;
+                ok = wait(q_full(h), q_phase[h], DEV_TIMEOUT_FULL);
+                q_phase[h] ^= 1u;
+                if (!ok) continue;
+                tc_fence_after_sync();
+                scores(h, stage);
+                if (it.n[h] == 1 && lane == 0) umma_commit(q_empty(h));
+            }
+            if (!ok) break;
+            if (lane == 0) umma_commit(kv_empty(stage));
+            __syncwarp();
+            advance(stage, phase);
+            for (int j = 0; ok && j < n; ++j) {
+                const int v_stage = stage;
+                const uint32_t v_phase = phase;
+                advance(stage, phase);
+                const int k_stage = stage;
+                const uint32_t k_phase = phase;
+                ok = wait(kv_full(v_stage), v_phase, DEV_TIMEOUT_FULL);
+                if (!ok) break;
+                const uint32_t v = base + L::kKvOffset + v_stage * L::kTileBytes;
+                const int left = it.s.k_len - j * kAttnKeys;  // keys of the sequence from this tile on
+                if (left < kAttnKeys && (left & 15)) {
+                    // rows behind the last key, up to the next 16: zeros (16 bytes per lane and step)
+                    const int rows = 16 - (left & 15);
+                    for (int e = lane; e < rows * 8 * (D / 64); e += 32) {
+                        const int box = e / (rows * 8), r = e % (rows * 8);
+                        *reinterpret_cast<uint4*>(smem + (v - base) + box * L::kBoxBytes + (left + r / 8) * 128 + (r % 8) * 16) =
+                            make_uint4(0u, 0u, 0u, 0u);
+                    }
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                }
+                const bool more = j + 1 < n;
+                if (more) ok = wait(kv_full(k_stage), k_phase, DEV_TIMEOUT_FULL);
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    if (!ok || j >= it.n[h]) continue;
+                    ok = wait(p_full(h), p_phase[h], DEV_TIMEOUT_TMEM_EMPTY);
+                    p_phase[h] ^= 1u;
+                    if (!ok) continue;
+                    tc_fence_after_sync();
+                    if (lane == 0) {
+                        // weights behind the tile's last visible key are zeros: those k-steps are left out
+                        int keys = left;
+                        if (p.causal) {
+                            const int last = min(it.t0 + (h + 1) * tile_tokens, it.s.q_len);
+                            keys = min(keys, last + it.s.k_len - it.s.q_len - j * kAttnKeys);
+                        }
+                        const int steps = min(kAttnKeys / 16, (keys + 15) / 16);
+                        const uint64_t v_desc = umma_smem_desc_sw128_mn(v, L::kBoxBytes);
+                        for (int x = 0; x < steps; ++x)  // 16 keys = 2048 bytes further in V, 8 columns in P
+                            umma_f16_ts(tmem + kO + h * 128, tmem + h * 128 + 8 * x, v_desc + 128u * x, idesc_o,
+                                        (j != 0 || x != 0) ? 1u : 0u);
+                        if (j == it.n[h] - 1) umma_commit(o_full(h));
+                    }
+                    if (j + 1 < it.n[h]) {
+                        scores(h, k_stage);
+                        if (j + 2 == it.n[h] && lane == 0) umma_commit(q_empty(h));
+                    }
+                    __syncwarp();
+                }
+                if (!ok) break;
+                if (lane == 0) {
+                    umma_commit(kv_empty(v_stage));
+                    if (more) umma_commit(kv_empty(k_stage));
+                }
+                __syncwarp();
+                if (more) advance(stage, phase);
+            }
+        }
+    } else {
+        // ---------------- softmax ----------------
+        const int h = warp >> 2, r = threadIdx.x & 127;
+        const uint32_t t_lane = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+        const uint32_t t_s = t_lane + h * 128, t_o = t_lane + kO + h * 128;
+        const int token = r / group, head_in = r - token * group;
+        uint32_t s_phase = 0, o_phase = 0;
+        bool ok = true;
+        for (int round = 0; ok && walk.find(p, attn_index(round), tile_tokens, lane, it); ++round) {
+            const int first = it.t0 + h * tile_tokens;
+            if (first >= it.s.q_len) continue;  // this tile has no rows
+            const int t = first + token;
+            const bool live = token < tile_tokens && t < it.s.q_len;
+            int limit = it.s.k_len, tile_limit = it.s.k_len;  // keys this row sees; keys every row of the tile sees
+            if (p.causal) {
+                limit = min(limit, max(0, t + 1 + it.s.k_len - it.s.q_len));
+                tile_limit = min(tile_limit, max(0, first + 1 + it.s.k_len - it.s.q_len));
+            }
+            const int n = h ? it.n[1] : it.n[0];
+            float m = -INFINITY, l = 0.0f;
+            for (int j = 0; j < n; ++j) {
+                ok = wait(s_full(h), s_phase, DEV_TIMEOUT_TMEM_FULL);
+                s_phase ^= 1u;
+                if (!ok) break;
+                tc_fence_after_sync();
+                uint32_t s[4][32];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) tmem_ld_32x32(t_s + 32 * c, s[c]);
+                tmem_ld_wait();
+                if ((j + 1) * kAttnKeys > tile_limit) {
+                    const int lim = limit - j * kAttnKeys;
+#pragma unroll
+                    for (int c = 0; c < 4; ++c)
+#pragma unroll
+                        for (int i = 0; i < 32; ++i)
+                            if (32 * c + i >= lim) s[c][i] = 0xff800000u;
+                }
+                float mx[4];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    mx[c] = __uint_as_float(s[c][0]);
+#pragma unroll
+                    for (int i = 1; i < 32; ++i) mx[c] = fmaxf(mx[c], __uint_as_float(s[c][i]));
+                }
+                const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                if (j == 0) {
+                    m = top;
+                } else if (__any_sync(0xffffffffu, (top - m) * p.scale_log2 > 8.0f || (m == -INFINITY && top > m))) {
+                    // the scores of this tile follow the product that last added to O: O is at rest
+                    const float up = fmaxf(m, top);
+                    const float keep = m == -INFINITY ? 0.0f : ex2((m - up) * p.scale_log2);
+                    m = up;
+                    l *= keep;
+#pragma unroll 1
+                    for (int c = 0; c < D; c += 32) {
+                        uint32_t o[32];
+                        tmem_ld_32x32(t_o + c, o);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * keep);
+                        tmem_st_32x32(t_o + c, o);
+                    }
+                }
+                const float off = m == -INFINITY ? 0.0f : -m * p.scale_log2;
+                float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int c = 0; c < 4; c += 2) {
+                    uint32_t w[32];
+#pragma unroll
+                    for (int i = 0; i < 32; i += 2) {
+                        const float a0 = ex2(fmaf(__uint_as_float(s[c][i]), p.scale_log2, off));
+                        const float a1 = ex2(fmaf(__uint_as_float(s[c][i + 1]), p.scale_log2, off));
+                        const float b0 = ex2(fmaf(__uint_as_float(s[c + 1][i]), p.scale_log2, off));
+                        const float b1 = ex2(fmaf(__uint_as_float(s[c + 1][i + 1]), p.scale_log2, off));
+                        sum[0] += a0, sum[1] += a1, sum[2] += b0, sum[3] += b1;
+                        w[i / 2] = pack2(a0, a1, TYPE);
+                        w[16 + i / 2] = pack2(b0, b1, TYPE);
+                    }
+                    tmem_st_32x32(t_s + 16 * c, w);
+                }
+                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                tmem_st_wait();
+                tc_fence_before_sync();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(p_full(h));
+            }
+            if (ok && n > 0) {
+                ok = wait(o_full(h), o_phase, DEV_TIMEOUT_TMEM_FULL);
+                o_phase ^= 1u;
+                tc_fence_after_sync();
+            }
+            if (!ok) break;
+            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+            const long long row = it.s.q0 + static_cast<long long>(t);
+            const int head = it.kv * group + head_in;
+#pragma unroll 1
+            for (int c = 0; c < D; c += 32) {
+                uint32_t o[32];
+                __syncwarp();
+                if (n > 0) {
+                    tmem_ld_32x32(t_o + c, o);
+                    tmem_ld_wait();
+                }
+                if (!live || c >= p.dim) continue;
+                uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + row * p.ld_out + static_cast<long long>(head) * p.dim + c);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if (c + 8 * i >= p.dim) break;
+                    uint32_t w[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        w[e] = l == 0.0f ? 0u
+                                         : pack2(__uint_as_float(o[8 * i + 2 * e]) * inv,
+                                                 __uint_as_float(o[8 * i + 2 * e + 1]) * inv, TYPE);
+                    dst[i] = make_uint4(w[0], w[1], w[2], w[3]);
+                }
+            }
+            if (live && p.lse)
+                p.lse[row * p.heads + head] = l == 0.0f ? -INFINITY : (m * p.scale_log2 + log2f(l)) * kLn2;
+            tc_fence_before_sync();  // O has been read: the weights of the next item may follow
+        }
+    }
+
+    __syncwarp();
+    if (*abort_flag) __nanosleep(1000000u);  // let bulk copies still in flight land before shared memory is released
+    tc_fence_before_sync();
+    __syncthreads();
+    tc_fence_after_sync();
+    if (warp == 8) tmem_dealloc(tmem, 512);
+}
+
+}  // namespace tk

@@ -1,6 +1,7 @@
 // C-ABI entry points of the decoder-block operators (the contracts are in include/tacker_b200.h).  Part of
 // tacker_b200.cu: uses its launch helpers and device state.
 #pragma once
+#include "attention_prompt.cuh"
 #include "attention_rows.cuh"
 #include "i8gemm.cuh"
 #include "row_ops.cuh"
@@ -117,6 +118,46 @@ static int i8_split(long long tiles, int kblocks, int sm_count, int most) {
     int s = 1;
     while (s < most && tiles * s * 2 <= sm_count && kblocks / (2 * s) >= 4) s *= 2;
     return s;
+}
+
+// 16-bit tensor [rows][heads][dim] with rows `ld` elements apart; box = 64 elements x box_heads x box_rows, 128-byte
+// swizzle; elements behind dim and rows behind the last arrive as zeros
+static int make_tmap_heads(CUtensorMap* m, const void* base, int type, int rows, int heads, int dim, long long ld,
+                           int box_heads, int box_rows) {
+    int rc = get_encoder();
+    if (rc != TK_OK) return rc;
+    cuuint64_t dims[3] = {static_cast<cuuint64_t>(dim), static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(rows)};
+    cuuint64_t strides[2] = {static_cast<cuuint64_t>(dim) * 2, static_cast<cuuint64_t>(ld) * 2};
+    cuuint32_t box[3] = {64, static_cast<cuuint32_t>(box_heads), static_cast<cuuint32_t>(box_rows)};
+    cuuint32_t estr[3] = {1, 1, 1};
+    CUresult r = g_encode(m, type == kBF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+                          const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) {
+        t_last_error = "cuTensorMapEncodeTiled (heads) failed with CUresult " + std::to_string(static_cast<int>(r));
+        return TK_ERR_CUDA;
+    }
+    return TK_OK;
+}
+
+template <int D, int TYPE>
+static int launch_attention_prompt(const AttnArgs& p, DeviceInfo* d, cudaStream_t st) {
+    auto kernel = attention_prompt_kernel<D, TYPE>;
+    constexpr int smem = AttnSmem<D>::kBytes + 1024;
+    static_assert(smem <= kMaxDynSmem, "shared memory of a CTA");
+    int rc = enable_smem(kernel, smem);
+    if (rc != TK_OK) return rc;
+    const int group = p.heads / p.kv_heads, tile_tokens = 128 / group;
+    CUtensorMap tq, tk_, tv;
+    if ((rc = make_tmap_heads(&tq, p.q, p.type, p.total_q, p.heads, p.dim, p.ld_q, group, tile_tokens)) != TK_OK) return rc;
+    if ((rc = make_tmap_heads(&tk_, p.k, p.type, p.kv_rows, p.kv_heads, p.dim, p.ld_k, 1, kAttnKeys)) != TK_OK) return rc;
+    if ((rc = make_tmap_heads(&tv, p.v, p.type, p.kv_rows, p.kv_heads, p.dim, p.ld_v, 1, kAttnKeys)) != TK_OK) return rc;
+    // no more items than this, whatever the lengths are
+    const long long items = (p.total_q / (2ll * tile_tokens) + p.n_seqs) * p.kv_heads;
+    const unsigned grid = static_cast<unsigned>(items < d->sm_count ? items : d->sm_count);
+    kernel<<<grid, kAttnThreads, smem, st>>>(tq, tk_, tv, p, group, d->status_ptr);
+    return launch_error("attention_prompt_kernel launch");
 }
 
 }  // namespace tk
@@ -311,6 +352,18 @@ TK_API int tk_attention_packed(const void* q, long long ld_q, const void* k, lon
     p.type = type, p.causal = causal, p.scale_log2 = scale * kLog2e;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     (void)workspace_bytes;
+    const int group = heads / kv_heads;
+    // what the tensor maps take: 16-byte rows of whole heads, a group within one tile, at least one key row
+    const bool tiles = dim % 8 == 0 && dim <= 128 && group <= 128 && kv_rows > 0 && ld_q % 8 == 0 && ld_k % 8 == 0 &&
+                       ld_v % 8 == 0 && ld_out % 8 == 0 && aligned16({q, k, v, out}) && p.scale_log2 > 1e-30f &&
+                       p.scale_log2 < 1e30f;
+    if (tiles) {
+        DeviceInfo* d = nullptr;
+        if ((rc = device_info(&d)) != TK_OK) return rc;
+        if (dim <= 64)
+            return type == kF16 ? launch_attention_prompt<64, kF16>(p, d, st) : launch_attention_prompt<64, kBF16>(p, d, st);
+        return type == kF16 ? launch_attention_prompt<128, kF16>(p, d, st) : launch_attention_prompt<128, kBF16>(p, d, st);
+    }
     const long long blocks = (static_cast<long long>(total_q) * heads + 3) / 4;
     if (blocks > kMaxGridX) return TK_ERR_SHAPE;
     if (dim <= 128)
