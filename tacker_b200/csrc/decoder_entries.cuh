@@ -3,6 +3,7 @@
 #pragma once
 #include "attention_prompt.cuh"
 #include "attention_rows.cuh"
+#include "attention_tokens.cuh"
 #include "i8gemm.cuh"
 #include "row_ops.cuh"
 
@@ -141,6 +142,8 @@ static int make_tmap_heads(CUtensorMap* m, const void* base, int type, int rows,
     return TK_OK;
 }
 
+constexpr int kTokenRows = 64;  // most rows (tokens x heads of a group) of a sequence for the token form
+
 template <int D, int TYPE>
 static int launch_attention_prompt(const AttnArgs& p, DeviceInfo* d, cudaStream_t st) {
     auto kernel = attention_prompt_kernel<D, TYPE>;
@@ -158,6 +161,58 @@ static int launch_attention_prompt(const AttnArgs& p, DeviceInfo* d, cudaStream_
     const unsigned grid = static_cast<unsigned>(items < d->sm_count ? items : d->sm_count);
     kernel<<<grid, kAttnThreads, smem, st>>>(tq, tk_, tv, p, group, d->status_ptr);
     return launch_error("attention_prompt_kernel launch");
+}
+
+// ranges of the key axis for the token form: a full device of CTAs (two per SM), or several rounds of them where the
+// lengths may differ; no range shorter than 256 keys; what the workspace holds
+static int token_splits(long long base, int max_k, int slots, size_t row_bytes, size_t workspace_bytes) {
+    long long s = base >= slots ? (4ll * slots + base - 1) / base : slots / base;
+    s = std::min(s, (static_cast<long long>(max_k) + 255) / 256);
+    s = std::min(s, static_cast<long long>(workspace_bytes / row_bytes));
+    return static_cast<int>(std::max(1ll, std::min(s, 1024ll)));
+}
+
+template <int D, int TYPE>
+static int launch_attention_tokens(const AttnArgs& p, DeviceInfo* d, int max_q, int max_k, void* workspace,
+                                   size_t workspace_bytes, cudaStream_t st) {
+    auto kernel = attention_tokens_kernel<D, TYPE>;
+    constexpr int smem = TokSmem<D>::kBytes + 1024;
+    static_assert(2 * (smem + 1024) <= kMaxDynSmem + 1024, "two CTAs per SM");
+    int rc = enable_smem(kernel, smem);
+    if (rc != TK_OK) return rc;
+    CUtensorMap tk_, tv;
+    if ((rc = make_tmap_heads(&tk_, p.k, p.type, p.kv_rows, p.kv_heads, p.dim, p.ld_k, 1, kTokKeys)) != TK_OK) return rc;
+    if ((rc = make_tmap_heads(&tv, p.v, p.type, p.kv_rows, p.kv_heads, p.dim, p.ld_v, 1, kTokKeys)) != TK_OK) return rc;
+    TokArgs a;
+    a.group = p.heads / p.kv_heads;
+    a.row_blocks = std::max(1, (std::min(max_q, p.total_q) * a.group + kTokRows - 1) / kTokRows);
+    const long long base = static_cast<long long>(p.n_seqs) * p.kv_heads * a.row_blocks;
+    const long long rows = static_cast<long long>(p.total_q) * p.heads;
+    const size_t row_bytes = static_cast<size_t>(rows) * (p.dim * sizeof(float) + sizeof(float2));
+    a.splits = token_splits(base, max_k, 2 * d->sm_count, row_bytes, workspace ? workspace_bytes : 0);
+    a.part_ml = static_cast<float2*>(workspace);
+    // the sums first: their size is a multiple of 8 bytes, rounded up to 16 for the vectors behind
+    a.part_o = reinterpret_cast<float*>(static_cast<char*>(workspace) + (static_cast<size_t>(rows) * a.splits * 8 + 15) / 16 * 16);
+    while (a.splits > 1 && static_cast<size_t>(reinterpret_cast<char*>(a.part_o) - static_cast<char*>(workspace)) +
+                                   static_cast<size_t>(rows) * a.splits * p.dim * 4 > workspace_bytes) {
+        --a.splits;
+        a.part_o = reinterpret_cast<float*>(static_cast<char*>(workspace) + (static_cast<size_t>(rows) * a.splits * 8 + 15) / 16 * 16);
+    }
+    if (base * a.splits > kMaxGridX) return TK_ERR_SHAPE;
+    kernel<<<static_cast<unsigned>(base * a.splits), kTokWarps * 32, smem, st>>>(tk_, tv, p, a, d->status_ptr);
+    if (a.splits == 1) return launch_error("attention_tokens_kernel launch");
+    if ((rc = launch_error("attention_tokens_kernel launch")) != TK_OK) return rc;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(rows), 1, 1);
+    cfg.blockDim = dim3(32 * std::min(8, (a.splits + 3) / 4), 1, 1);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    TK_CUDA(cudaLaunchKernelEx(&cfg, attention_join_kernel<TYPE>, p, a));
+    return TK_OK;
 }
 
 }  // namespace tk
@@ -335,7 +390,7 @@ TK_API int tk_attention_packed(const void* q, long long ld_q, const void* k, lon
         return TK_ERR_ARGS;
     if (heads % kv_heads) return TK_ERR_ARGS;
     if (n_seqs == 0 || total_q == 0) return TK_OK;
-    if (dim > 256 || heads > 65535) return TK_ERR_SHAPE;
+    if (dim > 256 || static_cast<long long>(total_q) * heads > kMaxGridX) return TK_ERR_SHAPE;
     if (!q || !out || !q_start || !k_start || !k_len || (kv_rows > 0 && (!k || !v))) return TK_ERR_ARGS;
     if (ld_q < static_cast<long long>(heads) * dim || ld_out < static_cast<long long>(heads) * dim ||
         ld_k < static_cast<long long>(kv_heads) * dim || ld_v < static_cast<long long>(kv_heads) * dim)
@@ -360,6 +415,14 @@ TK_API int tk_attention_packed(const void* q, long long ld_q, const void* k, lon
     if (tiles) {
         DeviceInfo* d = nullptr;
         if ((rc = device_info(&d)) != TK_OK) return rc;
+        // few rows per sequence: the time is that of reading the keys and values
+        if (static_cast<long long>(max_q) * group <= kTokenRows) {
+            if (dim <= 64)
+                return type == kF16 ? launch_attention_tokens<64, kF16>(p, d, max_q, max_k, workspace, workspace_bytes, st)
+                                    : launch_attention_tokens<64, kBF16>(p, d, max_q, max_k, workspace, workspace_bytes, st);
+            return type == kF16 ? launch_attention_tokens<128, kF16>(p, d, max_q, max_k, workspace, workspace_bytes, st)
+                                : launch_attention_tokens<128, kBF16>(p, d, max_q, max_k, workspace, workspace_bytes, st);
+        }
         if (dim <= 64)
             return type == kF16 ? launch_attention_prompt<64, kF16>(p, d, st) : launch_attention_prompt<64, kBF16>(p, d, st);
         return type == kF16 ? launch_attention_prompt<128, kF16>(p, d, st) : launch_attention_prompt<128, kBF16>(p, d, st);

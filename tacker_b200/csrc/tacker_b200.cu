@@ -1,4 +1,5 @@
 // libtacker_b200.so: the C-ABI entry points (see include/tacker_b200.h for the contract).
+#include <algorithm>
 #include <cmath>
 #include <initializer_list>
 
