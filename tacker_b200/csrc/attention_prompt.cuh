@@ -68,8 +68,80 @@ __device__ __forceinline__ uint64_t umma_smem_desc_sw128_mn(uint32_t smem_addr, 
     return d;
 }
 
-constexpr int kAttnThreads = 320;
+constexpr int kAttnThreads = 384;  // the last two warps only give their registers away
 constexpr int kAttnKeys = 128;  // keys of a tile
+
+// Registers: launched with 168 a thread (3 warps per scheduler); the softmax warps take 208, the others keep 88:
+// 2 x 128 x 208 + 128 x 88 = 384 x 168.
+constexpr int kAttnSoftmaxRegs = 208, kAttnOtherRegs = 88;
+static_assert(256 * kAttnSoftmaxRegs + 128 * kAttnOtherRegs <= kAttnThreads * 168, "registers of the block");
+template <int N>
+__device__ __forceinline__ void more_registers() {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void fewer_registers() {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+
+// two fp32 operations per instruction
+__device__ __forceinline__ void fma2(float& x, float& y, float sx, float sy, float ax, float ay) {
+    asm("{\n"
+        ".reg .b64 v, w, c;\n"
+        "mov.b64 v, {%0, %1};\n"
+        "mov.b64 w, {%2, %3};\n"
+        "mov.b64 c, {%4, %5};\n"
+        "fma.rn.f32x2 v, v, w, c;\n"
+        "mov.b64 {%0, %1}, v;\n"
+        "}\n"
+        : "+f"(x), "+f"(y)
+        : "f"(sx), "f"(sy), "f"(ax), "f"(ay));
+}
+__device__ __forceinline__ void add2(float& x, float& y, float ax, float ay) {
+    asm("{\n"
+        ".reg .b64 v, w;\n"
+        "mov.b64 v, {%0, %1};\n"
+        "mov.b64 w, {%2, %3};\n"
+        "add.rn.f32x2 v, v, w;\n"
+        "mov.b64 {%0, %1}, v;\n"
+        "}\n"
+        : "+f"(x), "+f"(y)
+        : "f"(ax), "f"(ay));
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+
+__device__ __forceinline__ float max_of(const uint32_t (&s)[32]) {
+    float m0 = __uint_as_float(s[0]), m1 = __uint_as_float(s[1]);
+#pragma unroll
+    for (int i = 2; i < 30; i += 4) {
+        m0 = max3(m0, __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
+        m1 = max3(m1, __uint_as_float(s[i + 2]), __uint_as_float(s[i + 3]));
+    }
+    return max3(max3(m0, __uint_as_float(s[30]), __uint_as_float(s[31])), m1, m1);
+}
+__device__ __forceinline__ void hide_from(uint32_t (&s)[32], int limit) {
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+        if (i >= limit) s[i] = 0xff800000u;  // -infinity
+}
+// 32 weights 2^(scale s + off) of a row: their sums by fours and, rounded to the type, their pairs from w[at] on
+template <int TYPE>
+__device__ __forceinline__ void weights(const uint32_t (&s)[32], float scale, float off, float (&sum)[4], uint32_t (&w)[32],
+                                        const int at) {
+#pragma unroll
+    for (int i = 0; i < 32; i += 2) {
+        float x = __uint_as_float(s[i]), y = __uint_as_float(s[i + 1]);
+        fma2(x, y, scale, scale, off, off);
+        x = ex2(x), y = ex2(y);
+        if (i & 2) add2(sum[2], sum[3], x, y);
+        else add2(sum[0], sum[1], x, y);
+        w[at + i / 2] = pack2(x, y, TYPE);
+    }
+}
 
 template <int D>
 struct AttnSmem {
@@ -209,7 +281,9 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
         return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, status, code)) != 0;
     };
 
-    if (warp == 9) {
+    if (warp >= 8) {
+      fewer_registers<kAttnOtherRegs>();
+      if (warp == 9) {
         // ---------------- TMA producer ----------------
         int stage = 0;
         uint32_t phase = 0, q_phase[2] = {0, 0};
@@ -264,7 +338,7 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
             for (int h = 0; h < 2; ++h)
                 ok = ok && mbar_wait(q_empty(h), q_phase[h] ^ 1u, abort_flag, status, DEV_TIMEOUT_EMPTY);
         }
-    } else if (warp == 8) {
+      } else if (warp == 8) {
         // ---------------- MMA issuer ----------------
         const uint32_t fmt = TYPE == kBF16 ? (1u << 7) | (1u << 10) : 0u;  // A and B format: 0 = fp16, 1 = bf16
         const uint32_t idesc_s = umma_idesc_f16_f32(128, kAttnKeys) | fmt;
@@ -368,8 +442,10 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
                 if (more) advance(stage, phase);
             }
         }
+      }
     } else {
         // ---------------- softmax ----------------
+        more_registers<kAttnSoftmaxRegs>();
         const int h = warp >> 2, r = threadIdx.x & 127;
         const uint32_t t_lane = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
         const uint32_t t_s = t_lane + h * 128, t_o = t_lane + kO + h * 128;
@@ -393,26 +469,26 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
                 s_phase ^= 1u;
                 if (!ok) break;
                 tc_fence_after_sync();
-                uint32_t s[4][32];
-#pragma unroll
-                for (int c = 0; c < 4; ++c) tmem_ld_32x32(t_s + 32 * c, s[c]);
+                uint32_t s0[32], s1[32], s2[32], s3[32];  // 128 scores of the row
+                float top;
+                tmem_ld_32x32(t_s, s0);
+                tmem_ld_32x32(t_s + 32, s1);
                 tmem_ld_wait();
+                tmem_ld_32x32(t_s + 64, s2);
+                tmem_ld_32x32(t_s + 96, s3);
                 if ((j + 1) * kAttnKeys > tile_limit) {
                     const int lim = limit - j * kAttnKeys;
-#pragma unroll
-                    for (int c = 0; c < 4; ++c)
-#pragma unroll
-                        for (int i = 0; i < 32; ++i)
-                            if (32 * c + i >= lim) s[c][i] = 0xff800000u;
+                    tmem_ld_wait();
+                    hide_from(s0, lim);
+                    hide_from(s1, lim - 32);
+                    hide_from(s2, lim - 64);
+                    hide_from(s3, lim - 96);
+                    top = fmaxf(fmaxf(max_of(s0), max_of(s1)), fmaxf(max_of(s2), max_of(s3)));
+                } else {
+                    top = fmaxf(max_of(s0), max_of(s1));
+                    tmem_ld_wait();
+                    top = max3(top, max_of(s2), max_of(s3));
                 }
-                float mx[4];
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    mx[c] = __uint_as_float(s[c][0]);
-#pragma unroll
-                    for (int i = 1; i < 32; ++i) mx[c] = fmaxf(mx[c], __uint_as_float(s[c][i]));
-                }
-                const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
                 if (j == 0) {
                     m = top;
                 } else if (__any_sync(0xffffffffu, (top - m) * p.scale_log2 > 8.0f || (m == -INFINITY && top > m))) {
@@ -433,20 +509,17 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
                 }
                 const float off = m == -INFINITY ? 0.0f : -m * p.scale_log2;
                 float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                for (int c = 0; c < 4; c += 2) {
+                {
                     uint32_t w[32];
-#pragma unroll
-                    for (int i = 0; i < 32; i += 2) {
-                        const float a0 = ex2(fmaf(__uint_as_float(s[c][i]), p.scale_log2, off));
-                        const float a1 = ex2(fmaf(__uint_as_float(s[c][i + 1]), p.scale_log2, off));
-                        const float b0 = ex2(fmaf(__uint_as_float(s[c + 1][i]), p.scale_log2, off));
-                        const float b1 = ex2(fmaf(__uint_as_float(s[c + 1][i + 1]), p.scale_log2, off));
-                        sum[0] += a0, sum[1] += a1, sum[2] += b0, sum[3] += b1;
-                        w[i / 2] = pack2(a0, a1, TYPE);
-                        w[16 + i / 2] = pack2(b0, b1, TYPE);
-                    }
-                    tmem_st_32x32(t_s + 16 * c, w);
+                    weights<TYPE>(s0, p.scale_log2, off, sum, w, 0);
+                    weights<TYPE>(s1, p.scale_log2, off, sum, w, 16);
+                    tmem_st_32x32(t_s, w);
+                }
+                {
+                    uint32_t w[32];
+                    weights<TYPE>(s2, p.scale_log2, off, sum, w, 0);
+                    weights<TYPE>(s3, p.scale_log2, off, sum, w, 16);
+                    tmem_st_32x32(t_s + 32, w);
                 }
                 l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
                 tmem_st_wait();
