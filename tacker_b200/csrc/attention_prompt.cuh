@@ -29,8 +29,70 @@
 
 namespace tk {
 
-// D[tmem] (+)= A[tmem] * B[smem]: the weights come from tensor memory
-__device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
+// one lane of a full warp, always the same
+__device__ __forceinline__ bool elect_lane() {
+    uint32_t e;
+    asm volatile(
+        "{\n"
+        ".reg .pred p;\n"
+        "elect.sync _|p, 0xffffffff;\n"
+        "selp.u32 %0, 1, 0, p;\n"
+        "}\n"
+        : "=r"(e));
+    return e != 0;
+}
+
+// The MMAs of a tile are issued back to back from one block of instructions: with N = 128 each takes 64 cycles of the
+// tensor pipe, and a loop that rebuilds its operands for each (138 cycles per MMA as measured) leaves the pipe idle.
+// Four k-steps of S = Q K^T: 16 elements = 32 bytes further along both swizzled rows
+__device__ __forceinline__ void umma_scores_x4(uint32_t d_tmem, uint64_t q_desc, uint64_t k_desc, uint32_t idesc,
+                                               uint32_t accumulate) {
+    asm volatile(
+        "{\n"
+        ".reg .pred p, t;\n"
+        ".reg .b64 a, b;\n"
+        "setp.ne.b32 p, %4, 0;\n"
+        "setp.eq.b32 t, 0, 0;\n"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n"
+        "add.s64 a, %1, 2;\n"
+        "add.s64 b, %2, 2;\n"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, t;\n"
+        "add.s64 a, %1, 4;\n"
+        "add.s64 b, %2, 4;\n"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, t;\n"
+        "add.s64 a, %1, 6;\n"
+        "add.s64 b, %2, 6;\n"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, t;\n"
+        "}\n" ::"r"(d_tmem),
+        "l"(q_desc), "l"(k_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+// Four k-steps of O += P V, P in tensor memory: 16 keys = 8 columns of P and 2048 bytes of V
+__device__ __forceinline__ void umma_values_x4(uint32_t d_tmem, uint32_t p_tmem, uint64_t v_desc, uint32_t idesc,
+                                               uint32_t accumulate) {
+    asm volatile(
+        "{\n"
+        ".reg .pred p, t;\n"
+        ".reg .b64 b;\n"
+        ".reg .b32 a;\n"
+        "setp.ne.b32 p, %4, 0;\n"
+        "setp.eq.b32 t, 0, 0;\n"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n"
+        "add.s32 a, %1, 8;\n"
+        "add.s64 b, %2, 128;\n"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [a], b, %3, t;\n"
+        "add.s32 a, %1, 16;\n"
+        "add.s64 b, %2, 256;\n"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [a], b, %3, t;\n"
+        "add.s32 a, %1, 24;\n"
+        "add.s64 b, %2, 384;\n"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [a], b, %3, t;\n"
+        "}\n" ::"r"(d_tmem),
+        "r"(p_tmem), "l"(v_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+// one k-step of O += P V
+__device__ __forceinline__ void umma_values(uint32_t d_tmem, uint32_t p_tmem, uint64_t v_desc, uint32_t idesc,
                                             uint32_t accumulate) {
     asm volatile(
         "{\n"
@@ -38,7 +100,7 @@ __device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, ui
         "setp.ne.b32 p, %4, 0;\n"
         "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n"
         "}\n" ::"r"(d_tmem),
-        "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        "r"(p_tmem), "l"(v_desc), "r"(idesc), "r"(accumulate)
         : "memory");
 }
 
@@ -229,7 +291,8 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
     constexpr uint32_t kO = 256;  // TMEM: S / P of tile 0 at column 0, of tile 1 at 128, O of the tiles at 256 and 384
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = align_smem_1024(smem_raw);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    // values that are the same in a whole warp are taken from lane 0, so that the compiler knows it
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const uint32_t base = smem_u32(smem);
     const uint32_t bars = base + L::kBarOffset;
     auto kv_full = [&](int s) { return bars + 8u * s; };
@@ -270,7 +333,7 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
     tc_fence_before_sync();
     __syncthreads();
     tc_fence_after_sync();
-    const uint32_t tmem = *tmem_slot;
+    const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
     const int tile_tokens = 128 / group;
 
     AttnWalk walk;
@@ -352,15 +415,15 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
                 ph ^= 1u;
             }
         };
+        const bool leader = elect_lane();
         auto scores = [&](int h, int st) {
-            if (lane == 0) {
-                const uint32_t q = base + h * L::kTileBytes, k = base + L::kKvOffset + st * L::kTileBytes;
+            const uint64_t q_desc = umma_smem_desc_sw128(base + h * L::kTileBytes);
+            const uint64_t k_desc = umma_smem_desc_sw128(base + L::kKvOffset + st * L::kTileBytes);
+            if (leader) {
 #pragma unroll
-                for (int x = 0; x < D / 16; ++x) {
-                    const uint32_t off = (x >> 2) * L::kBoxBytes;
-                    umma_f16(tmem + h * 128, umma_smem_desc_sw128(q + off) + 2u * (x & 3),
-                             umma_smem_desc_sw128(k + off) + 2u * (x & 3), idesc_s, x != 0);
-                }
+                for (int x = 0; x < D / 64; ++x)
+                    umma_scores_x4(tmem + h * 128, q_desc + x * (L::kBoxBytes >> 4), k_desc + x * (L::kBoxBytes >> 4),
+                                   idesc_s, x != 0);
                 umma_commit(s_full(h));
             }
         };
@@ -377,10 +440,10 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
                 if (!ok) continue;
                 tc_fence_after_sync();
                 scores(h, stage);
-                if (it.n[h] == 1 && lane == 0) umma_commit(q_empty(h));
+                if (it.n[h] == 1 && leader) umma_commit(q_empty(h));
             }
             if (!ok) break;
-            if (lane == 0) umma_commit(kv_empty(stage));
+            if (leader) umma_commit(kv_empty(stage));
             __syncwarp();
             advance(stage, phase);
             for (int j = 0; ok && j < n; ++j) {
@@ -413,28 +476,33 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
                     p_phase[h] ^= 1u;
                     if (!ok) continue;
                     tc_fence_after_sync();
-                    if (lane == 0) {
-                        // weights behind the tile's last visible key are zeros: those k-steps are left out
-                        int keys = left;
-                        if (p.causal) {
-                            const int last = min(it.t0 + (h + 1) * tile_tokens, it.s.q_len);
-                            keys = min(keys, last + it.s.k_len - it.s.q_len - j * kAttnKeys);
+                    // weights behind the tile's last visible key are zeros: those k-steps are left out
+                    int keys = left;
+                    if (p.causal) {
+                        const int last = min(it.t0 + (h + 1) * tile_tokens, it.s.q_len);
+                        keys = min(keys, last + it.s.k_len - it.s.q_len - j * kAttnKeys);
+                    }
+                    const uint64_t v_desc = umma_smem_desc_sw128_mn(v, L::kBoxBytes);
+                    const uint32_t o_tmem = tmem + kO + h * 128, p_tmem = tmem + h * 128;
+                    const int steps = (keys + 15) / 16;
+                    if (leader) {
+                        if (steps >= kAttnKeys / 16) {
+                            umma_values_x4(o_tmem, p_tmem, v_desc, idesc_o, j != 0);
+                            umma_values_x4(o_tmem, p_tmem + 32, v_desc + 512, idesc_o, 1);
+                        } else {
+                            for (int x = 0; x < steps; ++x)
+                                umma_values(o_tmem, p_tmem + 8 * x, v_desc + 128 * x, idesc_o, j != 0 || x != 0);
                         }
-                        const int steps = min(kAttnKeys / 16, (keys + 15) / 16);
-                        const uint64_t v_desc = umma_smem_desc_sw128_mn(v, L::kBoxBytes);
-                        for (int x = 0; x < steps; ++x)  // 16 keys = 2048 bytes further in V, 8 columns in P
-                            umma_f16_ts(tmem + kO + h * 128, tmem + h * 128 + 8 * x, v_desc + 128u * x, idesc_o,
-                                        (j != 0 || x != 0) ? 1u : 0u);
                         if (j == it.n[h] - 1) umma_commit(o_full(h));
                     }
                     if (j + 1 < it.n[h]) {
                         scores(h, k_stage);
-                        if (j + 2 == it.n[h] && lane == 0) umma_commit(q_empty(h));
+                        if (j + 2 == it.n[h] && leader) umma_commit(q_empty(h));
                     }
                     __syncwarp();
                 }
                 if (!ok) break;
-                if (lane == 0) {
+                if (leader) {
                     umma_commit(kv_empty(v_stage));
                     if (more) umma_commit(kv_empty(k_stage));
                 }
