@@ -130,13 +130,13 @@ __device__ __forceinline__ uint64_t umma_smem_desc_sw128_mn(uint32_t smem_addr, 
     return d;
 }
 
-constexpr int kAttnThreads = 384;  // the last two warps only give their registers away
+constexpr int kAttnThreads = 512;
 constexpr int kAttnKeys = 128;  // keys of a tile
 
-// Registers: launched with 168 a thread (3 warps per scheduler); the softmax warps take 208, the others keep 88:
-// 2 x 128 x 208 + 128 x 88 = 384 x 168.
-constexpr int kAttnSoftmaxRegs = 208, kAttnOtherRegs = 88;
-static_assert(256 * kAttnSoftmaxRegs + 128 * kAttnOtherRegs <= kAttnThreads * 168, "registers of the block");
+// Registers: launched with 128 a thread; the softmax warps keep a row of scores each.
+constexpr int kAttnSoftmaxRegs = 192, kAttnOutRegs = 72, kAttnOtherRegs = 56;
+static_assert(256 * kAttnSoftmaxRegs + 128 * kAttnOutRegs + 128 * kAttnOtherRegs <= kAttnThreads * 128,
+              "registers of the block");
 template <int N>
 __device__ __forceinline__ void more_registers() {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
@@ -170,9 +170,15 @@ __device__ __forceinline__ void add2(float& x, float& y, float ax, float ay) {
         : "+f"(x), "+f"(y)
         : "f"(ax), "f"(ay));
 }
+// maxima that are NaN where an operand is
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float d;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+__device__ __forceinline__ float max2(float a, float b) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
     return d;
 }
 
@@ -185,12 +191,17 @@ __device__ __forceinline__ float max_of(const uint32_t (&s)[32]) {
     }
     return max3(max3(m0, __uint_as_float(s[30]), __uint_as_float(s[31])), m1, m1);
 }
+// scores from `limit` on become -infinity; the limit as a mask of bits, which the compiler turns into predicates by sevens
 __device__ __forceinline__ void hide_from(uint32_t (&s)[32], int limit) {
+    const uint32_t seen = limit >= 32 ? 0xffffffffu : limit <= 0 ? 0u : (1u << limit) - 1u;
 #pragma unroll
     for (int i = 0; i < 32; ++i)
-        if (i >= limit) s[i] = 0xff800000u;  // -infinity
+        if (!(seen & (1u << i))) s[i] = 0xff800000u;
 }
-// 32 weights 2^(scale s + off) of a row: their sums by fours and, rounded to the type, their pairs from w[at] on
+
+// 32 weights 2^(scale s + off) of a row: their sums by fours and, rounded to the type, their pairs from w[at] on.  (A share
+// of the powers as polynomials on the multiply-add pipes, 1/8 to 3/8 of them, gained nothing: the tiles take turns on the
+// special-function units, and at full load the clock is set by the power limit.)
 template <int TYPE>
 __device__ __forceinline__ void weights(const uint32_t (&s)[32], float scale, float off, float (&sum)[4], uint32_t (&w)[32],
                                         const int at) {
@@ -209,11 +220,17 @@ template <int D>
 struct AttnSmem {
     static constexpr int kBoxBytes = 128 * 128;  // 128 rows x 64 elements
     static constexpr int kTileBytes = (D / 64) * kBoxBytes;
-    static constexpr int kStages = D == 128 ? 5 : 10;
+    static constexpr int kStages = D == 128 ? 4 : 8;
     static constexpr int kKvOffset = 2 * kTileBytes;
-    static constexpr int kBarOffset = kKvOffset + kStages * kTileBytes;
-    // barriers: ring full / empty, Q full / empty per tile, S full, P full, O full per tile
-    static constexpr int kNumBars = 2 * kStages + 10;
+    static constexpr int kOutOffset = kKvOffset + kStages * kTileBytes;
+    static constexpr int kOutWarpBytes = 32 * D * 2;  // 32 rows of the output on their way out
+    static constexpr int kStatOffset = kOutOffset + 4 * kOutWarpBytes;  // maximum and sum of each row of both tiles
+    static constexpr int kItemOffset = kStatOffset + 2 * 128 * 8;
+    static constexpr int kClaimOffset = kItemOffset + 32;
+    static constexpr int kBarOffset = kClaimOffset + 16;
+    // barriers: ring full / empty; per tile Q full / empty, S full, first half of P, all of P, O full, statistics full,
+    // O and statistics empty; item full / empty; claim
+    static constexpr int kNumBars = 2 * kStages + 16 + 3;
     static constexpr int kTmemSlotOffset = kBarOffset + kNumBars * 8;
     static constexpr int kAbortOffset = kTmemSlotOffset + 4;
     static constexpr int kBytes = kAbortOffset + 4;
@@ -230,55 +247,79 @@ struct AttnItem {
 // Finds work items by index, in ascending order of calls.  Items of a sequence run from its last tokens (which see the
 // most keys) to its first, key heads innermost.  All lanes of a warp call it together.
 struct AttnWalk {
-    int base;         // first sequence of the window of 32 that the search stands at
-    long long before; // items of the sequences before it
-    __device__ __forceinline__ void init() { base = 0, before = 0; }
+    int base;          // first sequence of the window of 32 that the search stands at; this lane's sequence is base + lane
+    AttnSeq s;
+    long long before;  // items of the sequences before the window
+    long long mine, upto;  // items of this lane's sequence, and of the window up to and with it
 
+    __device__ __forceinline__ void window(const AttnArgs& p, int tile_tokens, int lane) {
+        s.q_len = 0, s.q0 = 0, s.k0 = 0, s.k_len = 0;
+        if (base + lane < p.n_seqs) s.load(p, base + lane);
+        mine = static_cast<long long>((s.q_len + 2 * tile_tokens - 1) / (2 * tile_tokens)) * p.kv_heads;
+        upto = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long u = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += u;
+        }
+    }
+    __device__ __forceinline__ void init(const AttnArgs& p, int tile_tokens, int lane) {
+        base = 0, before = 0;
+        window(p, tile_tokens, lane);
+    }
     __device__ __forceinline__ bool find(const AttnArgs& p, long long index, int tile_tokens, int lane, AttnItem& it) {
-        const int pair_tokens = 2 * tile_tokens;
-        while (base < p.n_seqs) {
-            AttnSeq s;
-            s.q_len = 0, s.q0 = 0, s.k0 = 0, s.k_len = 0;
-            if (base + lane < p.n_seqs) s.load(p, base + lane);
-            const long long mine = static_cast<long long>((s.q_len + pair_tokens - 1) / pair_tokens) * p.kv_heads;
-            long long upto = mine;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const long long u = __shfl_up_sync(0xffffffffu, upto, o);
-                if (lane >= o) upto += u;
-            }
-            const uint32_t hit = __ballot_sync(0xffffffffu, before + upto > index);
-            if (hit) {
-                const int l = __ffs(hit) - 1;
-                it.s.q0 = __shfl_sync(0xffffffffu, s.q0, l);
-                it.s.q_len = __shfl_sync(0xffffffffu, s.q_len, l);
-                it.s.k0 = __shfl_sync(0xffffffffu, s.k0, l);
-                it.s.k_len = __shfl_sync(0xffffffffu, s.k_len, l);
-                const long long of = __shfl_sync(0xffffffffu, mine, l);
-                const long long at = index - before - (__shfl_sync(0xffffffffu, upto, l) - of);
-                it.kv = static_cast<int>(at % p.kv_heads);
-                it.t0 = static_cast<int>((of - 1 - at) / p.kv_heads) * pair_tokens;
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const int first = it.t0 + h * tile_tokens;
-                    const int last = min(first + tile_tokens, it.s.q_len) - 1;
-                    int keys = it.s.k_len;
-                    if (p.causal) keys = min(keys, max(0, last + 1 + it.s.k_len - it.s.q_len));
-                    it.n[h] = last < first ? 0 : (keys + kAttnKeys - 1) / kAttnKeys;
-                }
-                return true;
-            }
+        uint32_t hit;
+        while ((hit = __ballot_sync(0xffffffffu, before + upto > index)) == 0u) {
             before += __shfl_sync(0xffffffffu, upto, 31);
             base += 32;
+            if (base >= p.n_seqs) return false;
+            window(p, tile_tokens, lane);
         }
-        return false;
+        const int l = __ffs(hit) - 1;
+        it.s.q0 = __shfl_sync(0xffffffffu, s.q0, l);
+        it.s.q_len = __shfl_sync(0xffffffffu, s.q_len, l);
+        it.s.k0 = __shfl_sync(0xffffffffu, s.k0, l);
+        it.s.k_len = __shfl_sync(0xffffffffu, s.k_len, l);
+        const long long of = __shfl_sync(0xffffffffu, mine, l);
+        const int at = static_cast<int>(index - before - (__shfl_sync(0xffffffffu, upto, l) - of));
+        it.kv = at % p.kv_heads;
+        it.t0 = (static_cast<int>(of) - 1 - at) / p.kv_heads * 2 * tile_tokens;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int first = it.t0 + h * tile_tokens;
+            const int last = min(first + tile_tokens, it.s.q_len) - 1;
+            int keys = it.s.k_len;
+            if (p.causal) keys = min(keys, max(0, last + 1 + it.s.k_len - it.s.q_len));
+            it.n[h] = last < first ? 0 : (keys + kAttnKeys - 1) / kAttnKeys;
+        }
+        return true;
     }
 };
 
-// item of CTA c in round r: every other round runs backwards, so that long and short items even out
-__device__ __forceinline__ long long attn_index(int round) {
-    const long long g = gridDim.x;
-    return round * g + ((round & 1) ? g - 1 - blockIdx.x : static_cast<long long>(blockIdx.x));
+// ---- cluster launch control: take over a block of this grid that has not started -------------------------------------
+__device__ __forceinline__ void claim_request(uint32_t result_smem, uint32_t bar) {
+    asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(
+                     result_smem),
+                 "r"(bar)
+                 : "memory");
+}
+// the block taken over, or -1 when all have started
+__device__ __forceinline__ int claim_result(uint32_t result_smem) {
+    int x;
+    asm volatile(
+        "{\n"
+        ".reg .pred p;\n"
+        ".reg .b128 r;\n"
+        ".reg .b32 y, z, w;\n"
+        "ld.shared.b128 r, [%1];\n"
+        "mov.s32 %0, -1;\n"
+        "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\n"
+        "@p clusterlaunchcontrol.query_cancel.get_first_ctaid.v4.b32.b128 {%0, y, z, w}, r;\n"
+        "}\n"
+        : "=r"(x)
+        : "r"(result_smem)
+        : "memory");
+    return x;
 }
 
 template <int D, int TYPE>
@@ -289,8 +330,8 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
     using L = AttnSmem<D>;
     constexpr int ST = L::kStages;
     constexpr uint32_t kO = 256;  // TMEM: S / P of tile 0 at column 0, of tile 1 at 128, O of the tiles at 256 and 384
-    extern __shared__ uint8_t smem_raw[];
-    uint8_t* smem = align_smem_1024(smem_raw);
+    extern __shared__ __align__(1024) uint8_t attn_smem[];  // tiles need it; there is no room to align by hand
+    uint8_t* smem = attn_smem;
     // values that are the same in a whole warp are taken from lane 0, so that the compiler knows it
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const uint32_t base = smem_u32(smem);
@@ -300,12 +341,16 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
     auto q_full = [&](int h) { return bars + 8u * (2 * ST + h); };
     auto q_empty = [&](int h) { return bars + 8u * (2 * ST + 2 + h); };
     auto s_full = [&](int h) { return bars + 8u * (2 * ST + 4 + h); };
-    auto p_full = [&](int h) { return bars + 8u * (2 * ST + 6 + h); };
-    auto o_full = [&](int h) { return bars + 8u * (2 * ST + 8 + h); };
+    auto p_half = [&](int h) { return bars + 8u * (2 * ST + 6 + h); };
+    auto p_full = [&](int h) { return bars + 8u * (2 * ST + 8 + h); };
+    auto o_full = [&](int h) { return bars + 8u * (2 * ST + 10 + h); };
+    auto stat_full = [&](int h) { return bars + 8u * (2 * ST + 12 + h); };
+    auto o_empty = [&](int h) { return bars + 8u * (2 * ST + 14 + h); };
+    const uint32_t item_full = bars + 8u * (2 * ST + 16), item_empty = item_full + 8, claim_bar = item_full + 16;
     volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + L::kTmemSlotOffset);
     volatile uint32_t* abort_flag = reinterpret_cast<volatile uint32_t*>(smem + L::kAbortOffset);
 
-    if (warp == 8) {
+    if (warp == 12) {
         if (lane == 0) {
             *abort_flag = 0u;
             for (int s = 0; s < ST; ++s) {
@@ -316,16 +361,22 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
                 mbar_init(q_full(h), 1);
                 mbar_init(q_empty(h), 1);
                 mbar_init(s_full(h), 1);
-                mbar_init(p_full(h), 4);  // one arrival per softmax warp
+                mbar_init(p_half(h), 4);  // one arrival per softmax warp of the tile
+                mbar_init(p_full(h), 4);
                 mbar_init(o_full(h), 1);
+                mbar_init(stat_full(h), 4);
+                mbar_init(o_empty(h), 4);  // one per output warp
             }
+            mbar_init(item_full, 1);
+            mbar_init(item_empty, 14);  // every warp that works on items
+            mbar_init(claim_bar, 1);
             fence_mbar_init();
         }
         __syncwarp();
         tmem_alloc(smem_u32(const_cast<uint32_t*>(tmem_slot)), 512);
         tmem_relinquish();
     }
-    if (warp == 9 && lane == 0) {
+    if (warp == 13 && lane == 0) {
         tma_prefetch_desc(&tmap_q);
         tma_prefetch_desc(&tmap_k);
         tma_prefetch_desc(&tmap_v);
@@ -336,29 +387,82 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
     const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
     const int tile_tokens = 128 / group;
 
-    AttnWalk walk;
-    walk.init();
-    AttnItem it;
     // a wait of a whole warp: one verdict for all lanes
     auto wait = [&](uint32_t bar, uint32_t parity, unsigned code) {
         return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, status, code)) != 0;
     };
+    // the next item, for the warps that work on items; false at the end
+    uint32_t item_phase = 0;
+    AttnItem it;
+    auto next_item = [&](bool release) {
+        if (!wait(item_full, item_phase, DEV_TIMEOUT_FULL)) return false;
+        const int4* src = reinterpret_cast<const int4*>(smem + L::kItemOffset);
+        const int4 a = src[0], b = src[1];
+        it.s.q0 = __shfl_sync(0xffffffffu, a.x, 0), it.s.q_len = __shfl_sync(0xffffffffu, a.y, 0);
+        it.s.k0 = __shfl_sync(0xffffffffu, a.z, 0), it.s.k_len = __shfl_sync(0xffffffffu, a.w, 0);
+        it.kv = __shfl_sync(0xffffffffu, b.x, 0), it.t0 = __shfl_sync(0xffffffffu, b.y, 0);
+        it.n[0] = __shfl_sync(0xffffffffu, b.z, 0), it.n[1] = __shfl_sync(0xffffffffu, b.w, 0);
+        __syncwarp();
+        if (release && lane == 0) mbar_arrive(item_empty);
+        item_phase ^= 1u;
+        return it.t0 >= 0;
+    };
 
-    if (warp >= 8) {
+    if (warp >= 12) {
       fewer_registers<kAttnOtherRegs>();
-      if (warp == 9) {
+      if (warp == 14) {
+        // ---------------- items ----------------
+        AttnWalk walk;
+        walk.init(p, tile_tokens, lane);
+        int index = blockIdx.x;
+        uint32_t claim_phase = 0;
+        bool ok = true, open = true;  // open: there may be blocks that have not started
+        auto claim = [&]() {
+            if (lane == 0) {
+                fence_proxy_async_smem();  // the last result has been read
+                mbar_arrive_expect_tx(claim_bar, 16);
+                claim_request(base + L::kClaimOffset, claim_bar);
+            }
+            __syncwarp();
+            if (!wait(claim_bar, claim_phase, DEV_TIMEOUT_FULL)) return false;
+            claim_phase ^= 1u;
+            const int taken = claim_result(base + L::kClaimOffset);
+            __syncwarp();
+            open = taken >= 0;
+            if (open && taken < index) walk.init(p, tile_tokens, lane);  // the walk only goes forward
+            index = taken;
+            return true;
+        };
+        while (ok) {
+            const bool found = walk.find(p, index, tile_tokens, lane, it);
+            if (lane == 0) {
+                int4* dst = reinterpret_cast<int4*>(smem + L::kItemOffset);
+                dst[0] = make_int4(it.s.q0, it.s.q_len, it.s.k0, it.s.k_len);
+                dst[1] = make_int4(it.kv, found ? it.t0 : -1, it.n[0], it.n[1]);
+                mbar_arrive(item_full);
+            }
+            if (!found) break;
+            // the next one is claimed when the loads of this one are on their way and everyone has read it: earlier, and
+            // a CTA that is at a long item would hold another that nobody else can take
+            ok = wait(item_empty, item_phase, DEV_TIMEOUT_EMPTY);
+            item_phase ^= 1u;
+            if (!ok) break;
+            ok = claim();
+            if (!open) index = 0x7fffffff;  // no block has this number: the walk ends
+        }
+        while (ok && open) ok = claim();  // blocks behind the last item need not start
+      } else if (warp == 13) {
         // ---------------- TMA producer ----------------
         int stage = 0;
-        uint32_t phase = 0, q_phase[2] = {0, 0};
+        uint32_t phase = 0, q_phase0 = 0, q_phase1 = 0;
         bool ok = true;
         const uint32_t q_bytes = static_cast<uint32_t>((D / 64) * tile_tokens * group * 128);
-        for (int round = 0; ok && walk.find(p, attn_index(round), tile_tokens, lane, it); ++round) {
+        while (ok && next_item(false)) {
             if (lane == 0) {
                 const int n = max(it.n[0], it.n[1]);
-                auto load_q = [&](int h) {
-                    if (it.n[h] == 0) return true;
-                    if (!mbar_wait(q_empty(h), q_phase[h] ^ 1u, abort_flag, status, DEV_TIMEOUT_EMPTY)) return false;
-                    q_phase[h] ^= 1u;
+                auto load_q = [&](int h, uint32_t& q_phase) {
+                    if (!mbar_wait(q_empty(h), q_phase ^ 1u, abort_flag, status, DEV_TIMEOUT_EMPTY)) return false;
+                    q_phase ^= 1u;
                     mbar_arrive_expect_tx(q_full(h), q_bytes);
 #pragma unroll
                     for (int x = 0; x < D; x += 64)
@@ -379,14 +483,15 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
                     }
                     return true;
                 };
-                ok = load_q(0);
+                if (it.n[0] > 0) ok = load_q(0, q_phase0);
                 for (int j = 0; ok && j < n; ++j) {
                     ok = load_kv(&tmap_k, j);
-                    if (ok && j == 0) ok = load_q(1);
+                    if (ok && j == 0 && it.n[1] > 0) ok = load_q(1, q_phase1);
                     ok = ok && load_kv(&tmap_v, j);
                 }
             }
             ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+            if (lane == 0) mbar_arrive(item_empty);
         }
         // the last commits arrive on the empty barriers asynchronously: the CTA must not retire before they have landed
         if (lane == 0) {
@@ -397,15 +502,18 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
                     phase ^= 1u;
                 }
             }
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-                ok = ok && mbar_wait(q_empty(h), q_phase[h] ^ 1u, abort_flag, status, DEV_TIMEOUT_EMPTY);
+            ok = ok && mbar_wait(q_empty(0), q_phase0 ^ 1u, abort_flag, status, DEV_TIMEOUT_EMPTY);
+            ok = ok && mbar_wait(q_empty(1), q_phase1 ^ 1u, abort_flag, status, DEV_TIMEOUT_EMPTY);
         }
-      } else if (warp == 8) {
+      } else if (warp == 12) {
         // ---------------- MMA issuer ----------------
+        // Tile 0 and tile 1 strictly in turn: their softmaxes then run half a period apart, one on the special-function
+        // units while the other waits for its products (two independent issuers let them fall into step, where the powers
+        // of both take 2048 cycles at a time: 275 instead of 235 us for the long prompt).
         const uint32_t fmt = TYPE == kBF16 ? (1u << 7) | (1u << 10) : 0u;  // A and B format: 0 = fp16, 1 = bf16
         const uint32_t idesc_s = umma_idesc_f16_f32(128, kAttnKeys) | fmt;
         const uint32_t idesc_o = umma_idesc_f16_f32(128, D) | fmt | (1u << 16);  // B = V is MN-major
+        const bool leader = elect_lane();
         int stage = 0;  // ring position: K_0 V_0 K_1 V_1 ... of one item after another
         uint32_t phase = 0, q_phase[2] = {0, 0}, p_phase[2] = {0, 0};
         bool ok = true;
@@ -415,7 +523,8 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
                 ph ^= 1u;
             }
         };
-        const bool leader = elect_lane();
+        // S = Q K^T of tile h with the keys at ring position st; P lies over S and has been read when S overwrites it: MMAs
+        // of one thread run in order
         auto scores = [&](int h, int st) {
             const uint64_t q_desc = umma_smem_desc_sw128(base + h * L::kTileBytes);
             const uint64_t k_desc = umma_smem_desc_sw128(base + L::kKvOffset + st * L::kTileBytes);
@@ -427,7 +536,7 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
                 umma_commit(s_full(h));
             }
         };
-        for (int round = 0; ok && walk.find(p, attn_index(round), tile_tokens, lane, it); ++round) {
+        while (ok && next_item(true)) {
             const int n = max(it.n[0], it.n[1]);
             if (n == 0) continue;
             // the first scores of both tiles
@@ -469,29 +578,39 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
                 }
                 const bool more = j + 1 < n;
                 if (more) ok = wait(kv_full(k_stage), k_phase, DEV_TIMEOUT_FULL);
+                const uint64_t v_desc = umma_smem_desc_sw128_mn(v, L::kBoxBytes);
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     if (!ok || j >= it.n[h]) continue;
-                    ok = wait(p_full(h), p_phase[h], DEV_TIMEOUT_TMEM_EMPTY);
-                    p_phase[h] ^= 1u;
-                    if (!ok) continue;
-                    tc_fence_after_sync();
                     // weights behind the tile's last visible key are zeros: those k-steps are left out
                     int keys = left;
                     if (p.causal) {
                         const int last = min(it.t0 + (h + 1) * tile_tokens, it.s.q_len);
                         keys = min(keys, last + it.s.k_len - it.s.q_len - j * kAttnKeys);
                     }
-                    const uint64_t v_desc = umma_smem_desc_sw128_mn(v, L::kBoxBytes);
-                    const uint32_t o_tmem = tmem + kO + h * 128, p_tmem = tmem + h * 128;
                     const int steps = (keys + 15) / 16;
+                    const uint32_t o_tmem = tmem + kO + h * 128, p_tmem = tmem + h * 128;
+                    ok = wait(p_half(h), p_phase[h], DEV_TIMEOUT_TMEM_EMPTY);
+                    if (!ok) continue;
+                    tc_fence_after_sync();
                     if (leader) {
-                        if (steps >= kAttnKeys / 16) {
+                        if (steps >= kAttnKeys / 32) {
                             umma_values_x4(o_tmem, p_tmem, v_desc, idesc_o, j != 0);
-                            umma_values_x4(o_tmem, p_tmem + 32, v_desc + 512, idesc_o, 1);
                         } else {
                             for (int x = 0; x < steps; ++x)
                                 umma_values(o_tmem, p_tmem + 8 * x, v_desc + 128 * x, idesc_o, j != 0 || x != 0);
+                        }
+                    }
+                    ok = wait(p_full(h), p_phase[h], DEV_TIMEOUT_TMEM_EMPTY);
+                    p_phase[h] ^= 1u;
+                    if (!ok) continue;
+                    tc_fence_after_sync();
+                    if (leader) {
+                        if (steps >= kAttnKeys / 16) {
+                            umma_values_x4(o_tmem, p_tmem + 32, v_desc + 512, idesc_o, 1);
+                        } else {
+                            for (int x = kAttnKeys / 32; x < steps; ++x)
+                                umma_values(o_tmem, p_tmem + 8 * x, v_desc + 128 * x, idesc_o, 1);
                         }
                         if (j == it.n[h] - 1) umma_commit(o_full(h));
                     }
@@ -511,23 +630,93 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
             }
         }
       }
+    } else if (warp >= 8) {
+        // ---------------- output ----------------
+        fewer_registers<kAttnOutRegs>();
+        const int w32 = (warp & 3) * 32, r = w32 + lane;  // this thread's row of a tile
+        uint8_t* stage = smem + L::kOutOffset + (warp & 3) * L::kOutWarpBytes;
+        const uint32_t by_group = (65536u + group - 1) / group;  // r / group = r * by_group >> 16 for r < 128
+        uint32_t o_phase[2] = {0, 0}, stat_phase[2] = {0, 0};
+        bool ok = true;
+        while (ok && next_item(true)) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int first = it.t0 + h * tile_tokens;
+                if (!ok || first >= it.s.q_len) continue;  // the tile has no rows
+                const int n = it.n[h];
+                ok = wait(stat_full(h), stat_phase[h], DEV_TIMEOUT_TMEM_FULL);
+                stat_phase[h] ^= 1u;
+                if (!ok) continue;
+                if (n > 0) {
+                    ok = wait(o_full(h), o_phase[h], DEV_TIMEOUT_TMEM_FULL);
+                    o_phase[h] ^= 1u;
+                    if (!ok) continue;
+                    tc_fence_after_sync();
+                }
+                const float2 ml = *reinterpret_cast<const float2*>(smem + L::kStatOffset + (h * 128 + r) * 8);
+                const float inv = ml.y == 0.0f ? 0.0f : 1.0f / ml.y;
+                // through shared memory, so that the bytes of a row are written by neighbouring lanes: a row per lane and
+                // store touches 32 lines with each instruction
+                const uint32_t t_o = tmem + (static_cast<uint32_t>(w32) << 16) + kO + h * 128;
+#pragma unroll 1
+                for (int c = 0; c < D; c += 32) {
+                    uint32_t o[32];
+                    if (n > 0) {
+                        tmem_ld_32x32(t_o + c, o);
+                        tmem_ld_wait();
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        uint32_t w[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            w[e] = ml.y == 0.0f ? 0u
+                                                : pack2(__uint_as_float(o[8 * i + 2 * e]) * inv,
+                                                        __uint_as_float(o[8 * i + 2 * e + 1]) * inv, TYPE);
+                        *reinterpret_cast<uint4*>(stage + lane * (D * 2) + (((c / 8 + i) ^ (lane & 7)) << 4)) =
+                            make_uint4(w[0], w[1], w[2], w[3]);
+                    }
+                }
+                const int token = static_cast<int>(r * by_group >> 16);
+                if (p.lse && token < tile_tokens && first + token < it.s.q_len)
+                    p.lse[(it.s.q0 + static_cast<long long>(first + token)) * p.heads + it.kv * group + r - token * group] =
+                        ml.y == 0.0f ? -INFINITY : (ml.x * p.scale_log2 + log2f(ml.y)) * kLn2;
+                tc_fence_before_sync();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(o_empty(h));  // O and the statistics have been read
+                // D / 8 lanes per row
+                constexpr int kLanes = D / 8, kRows = 32 / kLanes;
+                const int chunk = lane % kLanes;
+                if (chunk * 8 < p.dim) {
+                    uint16_t* out = static_cast<uint16_t*>(p.out) + (it.s.q0 + static_cast<long long>(first)) * p.ld_out +
+                                    static_cast<long long>(it.kv) * group * p.dim + chunk * 8;
+#pragma unroll 4
+                    for (int i = 0; i < 32 / kRows; ++i) {
+                        const int rr = i * kRows + lane / kLanes;
+                        const int tr = static_cast<int>((w32 + rr) * by_group >> 16);
+                        if (tr < tile_tokens && first + tr < it.s.q_len)
+                            *reinterpret_cast<uint4*>(out + tr * p.ld_out + (w32 + rr - tr * group) * p.dim) =
+                                *reinterpret_cast<const uint4*>(stage + rr * (D * 2) + ((chunk ^ (rr & 7)) << 4));
+                    }
+                }
+                __syncwarp();
+            }
+        }
     } else {
         // ---------------- softmax ----------------
         more_registers<kAttnSoftmaxRegs>();
         const int h = warp >> 2, r = threadIdx.x & 127;
         const uint32_t t_lane = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
         const uint32_t t_s = t_lane + h * 128, t_o = t_lane + kO + h * 128;
-        const int token = r / group, head_in = r - token * group;
+        const int token = r / group;
         uint32_t s_phase = 0, o_phase = 0;
         bool ok = true;
-        for (int round = 0; ok && walk.find(p, attn_index(round), tile_tokens, lane, it); ++round) {
+        while (ok && next_item(true)) {
             const int first = it.t0 + h * tile_tokens;
             if (first >= it.s.q_len) continue;  // this tile has no rows
-            const int t = first + token;
-            const bool live = token < tile_tokens && t < it.s.q_len;
             int limit = it.s.k_len, tile_limit = it.s.k_len;  // keys this row sees; keys every row of the tile sees
             if (p.causal) {
-                limit = min(limit, max(0, t + 1 + it.s.k_len - it.s.q_len));
+                limit = min(limit, max(0, first + token + 1 + it.s.k_len - it.s.q_len));
                 tile_limit = min(tile_limit, max(0, first + 1 + it.s.k_len - it.s.q_len));
             }
             const int n = h ? it.n[1] : it.n[0];
@@ -551,31 +740,37 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
                     hide_from(s1, lim - 32);
                     hide_from(s2, lim - 64);
                     hide_from(s3, lim - 96);
-                    top = fmaxf(fmaxf(max_of(s0), max_of(s1)), fmaxf(max_of(s2), max_of(s3)));
+                    top = max2(max2(max_of(s0), max_of(s1)), max2(max_of(s2), max_of(s3)));
                 } else {
-                    top = fmaxf(max_of(s0), max_of(s1));
+                    top = max2(max_of(s0), max_of(s1));
                     tmem_ld_wait();
                     top = max3(top, max_of(s2), max_of(s3));
                 }
                 if (j == 0) {
                     m = top;
-                } else if (__any_sync(0xffffffffu, (top - m) * p.scale_log2 > 8.0f || (m == -INFINITY && top > m))) {
-                    // the scores of this tile follow the product that last added to O: O is at rest
-                    const float up = fmaxf(m, top);
-                    const float keep = m == -INFINITY ? 0.0f : ex2((m - up) * p.scale_log2);
-                    m = up;
-                    l *= keep;
+                } else {
+                    // a row's own scores decide, so that its result does not depend on its neighbours'; true from -infinity
+                    // and for NaN as well
+                    const bool raise = !((top - m) * p.scale_log2 <= 8.0f);
+                    if (__any_sync(0xffffffffu, raise)) {
+                        // the scores of this tile follow the product that last added to O: O is at rest
+                        const float up = raise ? max2(m, top) : m;
+                        const float keep = !raise ? 1.0f : m == -INFINITY ? 0.0f : ex2((m - up) * p.scale_log2);
+                        m = up;
+                        l *= keep;
 #pragma unroll 1
-                    for (int c = 0; c < D; c += 32) {
-                        uint32_t o[32];
-                        tmem_ld_32x32(t_o + c, o);
-                        tmem_ld_wait();
+                        for (int c = 0; c < D; c += 32) {
+                            uint32_t o[32];
+                            tmem_ld_32x32(t_o + c, o);
+                            tmem_ld_wait();
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * keep);
-                        tmem_st_32x32(t_o + c, o);
+                            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * keep);
+                            tmem_st_32x32(t_o + c, o);
+                        }
                     }
                 }
-                const float off = m == -INFINITY ? 0.0f : -m * p.scale_log2;
+                // a maximum of +infinity or NaN makes every weight of the row NaN, as the definition does
+                const float off = m == -INFINITY ? 0.0f : m == INFINITY ? NAN : -m * p.scale_log2;
                 float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
                 {
                     uint32_t w[32];
@@ -583,6 +778,15 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
                     weights<TYPE>(s1, p.scale_log2, off, sum, w, 16);
                     tmem_st_32x32(t_s, w);
                 }
+                if (j == 0) {  // the item before has left O
+                    ok = wait(o_empty(h), o_phase ^ 1u, DEV_TIMEOUT_TMEM_EMPTY);
+                    if (!ok) break;
+                    tc_fence_after_sync();
+                }
+                tmem_st_wait();
+                tc_fence_before_sync();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(p_half(h));  // the product with the first 64 values may start
                 {
                     uint32_t w[32];
                     weights<TYPE>(s2, p.scale_log2, off, sum, w, 0);
@@ -595,40 +799,13 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
                 __syncwarp();
                 if (lane == 0) mbar_arrive(p_full(h));
             }
-            if (ok && n > 0) {
-                ok = wait(o_full(h), o_phase, DEV_TIMEOUT_TMEM_FULL);
-                o_phase ^= 1u;
-                tc_fence_after_sync();
-            }
+            if (ok && n == 0) ok = wait(o_empty(h), o_phase ^ 1u, DEV_TIMEOUT_TMEM_EMPTY);
             if (!ok) break;
-            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-            const long long row = it.s.q0 + static_cast<long long>(t);
-            const int head = it.kv * group + head_in;
-#pragma unroll 1
-            for (int c = 0; c < D; c += 32) {
-                uint32_t o[32];
-                __syncwarp();
-                if (n > 0) {
-                    tmem_ld_32x32(t_o + c, o);
-                    tmem_ld_wait();
-                }
-                if (!live || c >= p.dim) continue;
-                uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + row * p.ld_out + static_cast<long long>(head) * p.dim + c);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    if (c + 8 * i >= p.dim) break;
-                    uint32_t w[4];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        w[e] = l == 0.0f ? 0u
-                                         : pack2(__uint_as_float(o[8 * i + 2 * e]) * inv,
-                                                 __uint_as_float(o[8 * i + 2 * e + 1]) * inv, TYPE);
-                    dst[i] = make_uint4(w[0], w[1], w[2], w[3]);
-                }
-            }
-            if (live && p.lse)
-                p.lse[row * p.heads + head] = l == 0.0f ? -INFINITY : (m * p.scale_log2 + log2f(l)) * kLn2;
-            tc_fence_before_sync();  // O has been read: the weights of the next item may follow
+            o_phase ^= 1u;
+            if (m == -INFINITY) l = 0.0f;  // every key of the row scored -infinity
+            *reinterpret_cast<float2*>(smem + L::kStatOffset + (h * 128 + r) * 8) = make_float2(m, l);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(stat_full(h));
         }
     }
 
@@ -637,7 +814,7 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
     tc_fence_before_sync();
     __syncthreads();
     tc_fence_after_sync();
-    if (warp == 8) tmem_dealloc(tmem, 512);
+    if (warp == 12) tmem_dealloc(tmem, 512);
 }
 
 }  // namespace tk

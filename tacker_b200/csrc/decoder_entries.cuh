@@ -147,7 +147,7 @@ constexpr int kTokenRows = 64;  // most rows (tokens x heads of a group) of a se
 template <int D, int TYPE>
 static int launch_attention_prompt(const AttnArgs& p, DeviceInfo* d, cudaStream_t st) {
     auto kernel = attention_prompt_kernel<D, TYPE>;
-    constexpr int smem = AttnSmem<D>::kBytes + 1024;
+    constexpr int smem = AttnSmem<D>::kBytes;
     static_assert(smem <= kMaxDynSmem, "shared memory of a CTA");
     int rc = enable_smem(kernel, smem);
     if (rc != TK_OK) return rc;
@@ -158,8 +158,8 @@ static int launch_attention_prompt(const AttnArgs& p, DeviceInfo* d, cudaStream_
     if ((rc = make_tmap_heads(&tv, p.v, p.type, p.kv_rows, p.kv_heads, p.dim, p.ld_v, 1, kAttnKeys)) != TK_OK) return rc;
     // no more items than this, whatever the lengths are
     const long long items = (p.total_q / (2ll * tile_tokens) + p.n_seqs) * p.kv_heads;
-    const unsigned grid = static_cast<unsigned>(items < d->sm_count ? items : d->sm_count);
-    kernel<<<grid, kAttnThreads, smem, st>>>(tq, tk_, tv, p, group, d->status_ptr);
+    if (items > kMaxGridX) return TK_ERR_SHAPE;
+    kernel<<<static_cast<unsigned>(items), kAttnThreads, smem, st>>>(tq, tk_, tv, p, group, d->status_ptr);
     return launch_error("attention_prompt_kernel launch");
 }
 
