@@ -41,6 +41,19 @@ static int on_this_device(std::initializer_list<const void*> ps) {
     return TK_OK;
 }
 
+// The opt-in to large shared memory, once per kernel and device (the call takes 1.5 us; devices beyond 64 pay it each time).
+template <auto KERNEL>
+static int enable_smem_once(int bytes) {
+    static std::atomic<unsigned long long> done{0};
+    int dev = 0;
+    TK_CUDA(cudaGetDevice(&dev));
+    const unsigned long long bit = dev < 64 ? 1ull << dev : 0ull;
+    if (done.load(std::memory_order_acquire) & bit) return TK_OK;
+    TK_CUDA(cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    done.fetch_or(bit, std::memory_order_release);
+    return TK_OK;
+}
+
 static int pow2_at_least(long long n, int lo, int hi) {
     int p = lo;
     while (p < n && p < hi) p <<= 1;
@@ -49,22 +62,27 @@ static int pow2_at_least(long long n, int lo, int hi) {
 
 constexpr long long kMaxGridX = 0x7fffffffll;
 
-// threads per row and groups of eight columns per thread of the row kernels
+// threads per row of the row kernels (two groups of eight columns each), threads and blocks of the launch
 struct RowShape {
-    int tpr, nv, block;
-    unsigned grid;
+    int tpr, block;
+    long long blocks;
 };
 static RowShape row_shape(long long rows, int cols) {
     RowShape s;
-    const int groups = cols / 8;
-    s.tpr = pow2_at_least((groups + 1) / 2, 32, 1024);
-    s.nv = (groups + s.tpr - 1) / s.tpr;
+    s.tpr = pow2_at_least((cols / 8 + 1) / 2, 32, 1024);
     s.block = s.tpr < 128 ? 128 : s.tpr;
     const long long per = s.block / s.tpr;
-    s.grid = static_cast<unsigned>((rows + per - 1) / per);
+    s.blocks = (rows + per - 1) / per;
     return s;
 }
-constexpr int kRowRegisterCols = 1024 * 4 * 8;  // widest row the register form holds
+
+// a runtime element type as a template argument
+template <typename F>
+static int with_type(int type, F f) {
+    if (type == kF32) return f(std::integral_constant<int, kF32>());
+    if (type == kF16) return f(std::integral_constant<int, kF16>());
+    return f(std::integral_constant<int, kBF16>());
+}
 
 // 8-bit matrix [rows][k], k contiguous, leading dimension ld bytes; box = 128 bytes x box_rows, 128-byte swizzle
 static int make_tmap_i8(CUtensorMap* m, const void* base, int rows, int k, long long ld, int box_rows) {
@@ -87,9 +105,9 @@ static int make_tmap_i8(CUtensorMap* m, const void* base, int rows, int k, long 
 template <int BN, int STAGES, bool SWAP>
 static int launch_i8gemm(const void* A, long long lda, const void* B, long long ldb, const I8Args& p, int split,
                          cudaStream_t st) {
-    auto kernel = i8gemm_kernel<BN, STAGES, SWAP>;
+    constexpr auto kernel = i8gemm_kernel<BN, STAGES, SWAP>;
     constexpr int smem = I8Smem<BN, STAGES>::kBytes + 1024;
-    int rc = enable_smem(kernel, smem);
+    int rc = enable_smem_once<kernel>(smem);
     if (rc != TK_OK) return rc;
     const int rows_a = SWAP ? p.N : p.M, rows_b = SWAP ? p.M : p.N;
     CUtensorMap ta, tb;
@@ -146,10 +164,10 @@ constexpr int kTokenRows = 64;  // most rows (tokens x heads of a group) of a se
 
 template <int D, int TYPE>
 static int launch_attention_prompt(const AttnArgs& p, DeviceInfo* d, cudaStream_t st) {
-    auto kernel = attention_prompt_kernel<D, TYPE>;
+    constexpr auto kernel = attention_prompt_kernel<D, TYPE>;
     constexpr int smem = AttnSmem<D>::kBytes;
     static_assert(smem <= kMaxDynSmem, "shared memory of a CTA");
-    int rc = enable_smem(kernel, smem);
+    int rc = enable_smem_once<kernel>(smem);
     if (rc != TK_OK) return rc;
     const int group = p.heads / p.kv_heads, tile_tokens = 128 / group;
     CUtensorMap tq, tk_, tv;
@@ -175,10 +193,10 @@ static int token_splits(long long base, int max_k, int slots, size_t row_bytes, 
 template <int D, int TYPE>
 static int launch_attention_tokens(const AttnArgs& p, DeviceInfo* d, int max_q, int max_k, void* workspace,
                                    size_t workspace_bytes, cudaStream_t st) {
-    auto kernel = attention_tokens_kernel<D, TYPE>;
+    constexpr auto kernel = attention_tokens_kernel<D, TYPE>;
     constexpr int smem = TokSmem<D>::kBytes + 1024;
     static_assert(2 * (smem + 1024) <= kMaxDynSmem + 1024, "two CTAs per SM");
-    int rc = enable_smem(kernel, smem);
+    int rc = enable_smem_once<kernel>(smem);
     if (rc != TK_OK) return rc;
     CUtensorMap tk_, tv;
     if ((rc = make_tmap_heads(&tk_, p.k, p.type, p.kv_rows, p.kv_heads, p.dim, p.ld_k, 1, kTokKeys)) != TK_OK) return rc;
@@ -245,18 +263,26 @@ TK_API int tk_norm_residual_rows(const void* a, int a_type, long long ld_a, int 
     p.a_type = a_type, p.x_type = x_type, p.h_type = h_type, p.cols = cols, p.post = post, p.layer = layer;
     p.scale = scale, p.eps = eps;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const bool vec = cols % 8 == 0 && cols <= kRowRegisterCols && ld_a % 8 == 0 && (!x || ld_x % 8 == 0) &&
+    const bool vec = cols % 8 == 0 && cols <= kNormCols && ld_a % 8 == 0 && (!x || ld_x % 8 == 0) &&
                      (!y || ld_y % 8 == 0) && (!h || ld_h % 8 == 0) && (!gate || ld_gate % 4 == 0) &&
                      aligned16({a, x, y, h, gate, post_gamma, post_beta, pre_gamma, pre_beta});
     if (!vec) {
         norm_residual_any_kernel<<<static_cast<unsigned>(rows), 256, 0, st>>>(p);
         return launch_error("norm_residual_any_kernel launch");
     }
+    DeviceInfo* d = nullptr;
+    if ((rc = device_info(&d)) != TK_OK) return rc;
     const RowShape s = row_shape(rows, cols);
-    if (s.nv <= 1) norm_residual_kernel<1><<<s.grid, s.block, 0, st>>>(p, s.tpr);
-    else if (s.nv <= 2) norm_residual_kernel<2><<<s.grid, s.block, 0, st>>>(p, s.tpr);
-    else norm_residual_kernel<4><<<s.grid, s.block, 0, st>>>(p, s.tpr);
-    return launch_error("norm_residual_kernel launch");
+    // 64 registers a thread: 1024 threads per SM
+    const unsigned grid = static_cast<unsigned>(std::min(s.blocks, static_cast<long long>(d->sm_count) * (1024 / s.block)));
+    return with_type(a_type, [&](auto at) {
+        return with_type(x_type, [&](auto xt) {
+            return with_type(h_type, [&](auto ht) {
+                norm_residual_kernel<at.value, xt.value, ht.value><<<grid, s.block, 0, st>>>(p, s.tpr);
+                return launch_error("norm_residual_kernel launch");
+            });
+        });
+    });
 }
 
 TK_API int tk_quantize_rows_i8(const void* x, int x_type, long long ld_x, void* codes, long long ld_codes, float* scales,
@@ -272,15 +298,17 @@ TK_API int tk_quantize_rows_i8(const void* x, int x_type, long long ld_x, void* 
     p.x = x, p.codes = static_cast<int8_t*>(codes), p.scales = scales;
     p.ld_x = ld_x, p.ld_codes = ld_codes, p.rows = rows, p.type = x_type, p.cols = cols;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (cols % 8 || cols > kRowRegisterCols || ld_x % 8 || ld_codes % 8 || !aligned16({x}) || !aligned_to(codes, 8)) {
+    if (cols % 8 || cols > kQuantCols || ld_x % 8 || ld_codes % 8 || !aligned16({x}) || !aligned_to(codes, 8)) {
         quantize_rows_any_kernel<<<static_cast<unsigned>(rows), 256, 0, st>>>(p);
         return launch_error("quantize_rows_any_kernel launch");
     }
     const RowShape s = row_shape(rows, cols);
-    if (s.nv <= 1) quantize_rows_kernel<1><<<s.grid, s.block, 0, st>>>(p, s.tpr);
-    else if (s.nv <= 2) quantize_rows_kernel<2><<<s.grid, s.block, 0, st>>>(p, s.tpr);
-    else quantize_rows_kernel<4><<<s.grid, s.block, 0, st>>>(p, s.tpr);
-    return launch_error("quantize_rows_kernel launch");
+    const unsigned grid = static_cast<unsigned>(s.blocks);
+    return with_type(x_type, [&](auto xt) {
+        if (cols <= kNormCols) quantize_rows_kernel<2, xt.value><<<grid, s.block, 0, st>>>(p, s.tpr);
+        else quantize_rows_kernel<4, xt.value><<<grid, s.block, 0, st>>>(p, s.tpr);
+        return launch_error("quantize_rows_kernel launch");
+    });
 }
 
 TK_API int tk_i8gemm(const void* A, long long lda, const float* scale_a, const void* B, long long ldb,
@@ -373,11 +401,16 @@ TK_API int tk_rope_qkv(const void* x, int x_type, long long ld_x, const float* b
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const bool vec = dim % 16 == 0 && rot_dim % 16 == 0 && ld_x % 8 == 0 && ld_q % 8 == 0 && ld_k % 8 == 0 &&
                      ld_v % 8 == 0 && aligned16({x, bias, q, k, v});
-    if (vec)
-        rope_qkv_vec_kernel<<<static_cast<unsigned>(tokens), 128, 0, st>>>(p);
-    else
+    if (!vec) {
         rope_qkv_any_kernel<<<static_cast<unsigned>(tokens), 128, 0, st>>>(p);
-    return launch_error(vec ? "rope_qkv_vec_kernel launch" : "rope_qkv_any_kernel launch");
+        return launch_error("rope_qkv_any_kernel launch");
+    }
+    return with_type(x_type, [&](auto xt) {
+        return with_type(out_type, [&](auto ot) {
+            rope_qkv_vec_kernel<xt.value, ot.value><<<static_cast<unsigned>(tokens), 128, 0, st>>>(p);
+            return launch_error("rope_qkv_vec_kernel launch");
+        });
+    });
 }
 
 TK_API int tk_attention_packed(const void* q, long long ld_q, const void* k, long long ld_k, const void* v, long long ld_v,

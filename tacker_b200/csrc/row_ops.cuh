@@ -87,18 +87,18 @@ __device__ __forceinline__ void load8f(const float* p, int i, float (&v)[8]) {
     v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
 }
 
-// Sum over the `tpr` threads of a row (a power of two, at least a warp); `slot` is a shared array of one float per warp
-// of the block.  Every thread of the block calls it, the same number of times.
-__device__ __forceinline__ float row_sum(float v, int tpr, float* slot) {
+// Sum over the `tpr` threads of a row (a power of two, at least a warp).  `slots` is a shared array of 2 x 32 floats, used in
+// turn so that one barrier per sum is enough; `turn` counts the sums.  Every thread of the block calls it, the same number
+// of times.
+__device__ __forceinline__ float row_sum(float v, int tpr, float* slots, int& turn) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     if (tpr == 32) return v;
-    const int warp = threadIdx.x >> 5, per = tpr >> 5, first = warp / per * per;
-    __syncthreads();  // the slots of the sum before have been read
-    if ((threadIdx.x & 31) == 0) slot[warp] = v;
+    const int warp = threadIdx.x >> 5, per = tpr >> 5, first = warp / per * per, lane = threadIdx.x & 31;
+    float* slot = slots + 32 * (turn++ & 1);
+    if (lane == 0) slot[warp] = v;
     __syncthreads();
     // at most 32 warps share a row: one more butterfly over their partial sums, the same order in every warp
-    const int lane = threadIdx.x & 31;
     float s = lane < per ? slot[first + lane] : 0.0f;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
@@ -125,105 +125,113 @@ struct NormArgs {
     float scale, eps;
 };
 
-// One row per `tpr` threads, NV groups of eight columns per thread in registers.  x is fetched before the first sum so
-// that its latency and a's overlap.
-template <int NV>
-__global__ void norm_residual_kernel(const NormArgs p, const int tpr) {
-    __shared__ float slot[32];
-    const long long row = static_cast<long long>(blockIdx.x) * (blockDim.x / tpr) + threadIdx.x / tpr;
-    const int t = threadIdx.x & (tpr - 1);
-    const bool live = row < p.rows;
+// One row per `tpr` threads, two groups of eight columns per thread in registers; the blocks stay and walk over the rows,
+// with the next row's a and x on their way while this one is summed up.  The types are compile-time constants: chosen
+// at run time, the conversions alone were two thirds of 54 instructions per element and the kernel was bound by issue
+// (80 us at 8191 x 4096 bf16 instead of 48, of which memory needs 41).
+constexpr int kNormCols = 1024 * 2 * 8;  // widest row
+template <int AT, int XT, int HT>
+__global__ void __launch_bounds__(1024) norm_residual_kernel(const NormArgs p, const int tpr) {
+    __shared__ float slots[64];
+    const int per_block = blockDim.x / tpr, t = threadIdx.x & (tpr - 1);
+    const long long step = static_cast<long long>(gridDim.x) * per_block;
     const float inv_cols = 1.0f / static_cast<float>(p.cols);
-    float v[NV][8];
-    Raw8 xr[NV];
+    int turn = 0;
+    Raw8 ar[2], xr[2];
+    auto fetch = [&](const void* src, int type, long long ld, long long row, Raw8 (&r)[2]) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        const int c = (t + i * tpr) * 8;
-        if (live && c < p.cols) {
-            const Raw8 r = load_raw8(p.a, p.a_type, row * p.ld_a + c);
-            if (p.x) xr[i] = load_raw8(p.x, p.x_type, row * p.ld_x + c);
-            unpack8(r, p.a_type, v[i]);
-        } else {
+        for (int i = 0; i < 2; ++i) {
+            const int c = (t + i * tpr) * 8;
+            if (src && row < p.rows && c < p.cols) r[i] = load_raw8(src, type, row * ld + c);
+        }
+    };
+    long long row = static_cast<long long>(blockIdx.x) * per_block + threadIdx.x / tpr;
+    fetch(p.a, AT, p.ld_a, row, ar);
+    fetch(p.x, XT, p.ld_x, row, xr);
+    // all threads of a block make the same number of rounds, for the barriers in the sums
+    for (long long base = static_cast<long long>(blockIdx.x) * per_block; base < p.rows; base += step, row += step) {
+        const bool live = row < p.rows;
+        float v[2][8];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) v[i][j] = 0.0f;
+            if (live && (t + i * tpr) * 8 < p.cols) unpack8(ar[i], AT, v[i]);
         }
-    }
-    // v <- (v - mean) * rstd over the columns of the row; the padding columns stay out of the sums
-    auto normalise = [&]() {
-        float mean = 0.0f;
-        if (p.layer) {
-            float s = 0.0f;
+        fetch(p.a, AT, p.ld_a, row + step, ar);
+        // v <- (v - mean) * rstd over the columns of the row; the padding columns stay out of the sums
+        auto normalise = [&]() {
+            float mean = 0.0f;
+            if (p.layer) {
+                float s = 0.0f;
 #pragma unroll
-            for (int i = 0; i < NV; ++i)
+                for (int i = 0; i < 2; ++i)
 #pragma unroll
-                for (int j = 0; j < 8; ++j) s += v[i][j];
-            mean = row_sum(s, tpr, slot) * inv_cols;
-        }
-        float q = 0.0f;
+                    for (int j = 0; j < 8; ++j) s += v[i][j];
+                mean = row_sum(s, tpr, slots, turn) * inv_cols;
+            }
+            float q = 0.0f;
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            if ((t + i * tpr) * 8 < p.cols) {
+            for (int i = 0; i < 2; ++i) {
+                if ((t + i * tpr) * 8 < p.cols) {
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    v[i][j] -= mean;
-                    q = fmaf(v[i][j], v[i][j], q);
+                    for (int j = 0; j < 8; ++j) {
+                        v[i][j] -= mean;
+                        q = fmaf(v[i][j], v[i][j], q);
+                    }
                 }
             }
-        }
-        const float rstd = rsqrtf(row_sum(q, tpr, slot) * inv_cols + p.eps);
+            const float rstd = rsqrtf(row_sum(q, tpr, slots, turn) * inv_cols + p.eps);
 #pragma unroll
-        for (int i = 0; i < NV; ++i)
+            for (int i = 0; i < 2; ++i)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[i][j] *= rstd;
-    };
-    auto affine = [&](const float* gamma, const float* beta, int i, int c) {
-        if (gamma) {
+                for (int j = 0; j < 8; ++j) v[i][j] *= rstd;
+        };
+        auto affine = [&](const float* gamma, const float* beta, int i, int c) {
             float g[8];
-            load8f(gamma, c, g);
+            if (gamma) {
+                load8f(gamma, c, g);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[i][j] *= g[j];
+                for (int j = 0; j < 8; ++j) v[i][j] *= g[j];
+            }
+            if (beta) {
+                load8f(beta, c, g);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[i][j] += g[j];
+            }
+        };
+        if (p.post) normalise();
+        const float* gate = p.gate && live ? p.gate + row / p.gate_rows * p.ld_gate : nullptr;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int c = (t + i * tpr) * 8;
+            if (!live || c >= p.cols) continue;
+            if (p.post) affine(p.post_gamma, p.post_beta, i, c);
+            if (gate) affine(gate, nullptr, i, c);
+            float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+            if (p.x) unpack8(xr[i], XT, x);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[i][j] = fmaf(p.scale, v[i][j], x[j]);
+            if (p.y) store8(p.y, XT, row * p.ld_y + c, v[i]);
         }
-        if (beta) {
-            float b[8];
-            load8f(beta, c, b);
+        fetch(p.x, XT, p.ld_x, row + step, xr);
+        if (!p.h) continue;
+        normalise();
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[i][j] += b[j];
+        for (int i = 0; i < 2; ++i) {
+            const int c = (t + i * tpr) * 8;
+            if (!live || c >= p.cols) continue;
+            affine(p.pre_gamma, p.pre_beta, i, c);
+            store8(p.h, HT, row * p.ld_h + c, v[i]);
         }
-    };
-    if (p.post) normalise();
-    const float* gate = p.gate && live ? p.gate + row / p.gate_rows * p.ld_gate : nullptr;
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        const int c = (t + i * tpr) * 8;
-        if (!live || c >= p.cols) continue;
-        if (p.post) affine(p.post_gamma, p.post_beta, i, c);
-        if (gate) {
-            float g[8];
-            load8f(gate, c, g);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[i][j] *= g[j];
-        }
-        float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        if (p.x) unpack8(xr[i], p.x_type, x);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[i][j] = fmaf(p.scale, v[i][j], x[j]);
-        if (p.y) store8(p.y, p.x_type, row * p.ld_y + c, v[i]);
-    }
-    if (!p.h) return;
-    normalise();
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        const int c = (t + i * tpr) * 8;
-        if (!live || c >= p.cols) continue;
-        affine(p.pre_gamma, p.pre_beta, i, c);
-        store8(p.h, p.h_type, row * p.ld_h + c, v[i]);
     }
 }
 
 // Any width, stride and alignment: one block per row, each pass reads the row again (from L2 after the first).  y is
 // written in the last pass only, so that it may be x.
 __global__ void norm_residual_any_kernel(const NormArgs p) {
-    __shared__ float slot[32];
+    __shared__ float slots[64];
+    int turn = 0;
     const int tpr = blockDim.x;
     const long long row = blockIdx.x;
     const float inv_cols = 1.0f / static_cast<float>(p.cols);
@@ -233,14 +241,14 @@ __global__ void norm_residual_any_kernel(const NormArgs p) {
         if (p.layer) {
             float s = 0.0f;
             for (int c = threadIdx.x; c < p.cols; c += tpr) s += value(c);
-            mean = row_sum(s, tpr, slot) * inv_cols;
+            mean = row_sum(s, tpr, slots, turn) * inv_cols;
         }
         float q = 0.0f;
         for (int c = threadIdx.x; c < p.cols; c += tpr) {
             const float d = value(c) - mean;
             q = fmaf(d, d, q);
         }
-        rstd = rsqrtf(row_sum(q, tpr, slot) * inv_cols + p.eps);
+        rstd = rsqrtf(row_sum(q, tpr, slots, turn) * inv_cols + p.eps);
     };
     float m1 = 0.0f, r1 = 1.0f, m2 = 0.0f, r2 = 1.0f;
     if (p.post) stats([&](int c) { return load1(p.a, p.a_type, row * p.ld_a + c); }, m1, r1);
@@ -299,6 +307,8 @@ __device__ __forceinline__ uint32_t row_umax(uint32_t v, int tpr, uint32_t* slot
     return __reduce_max_sync(0xffffffffu, lane < per ? slot[first + lane] : 0u);
 }
 
+constexpr int kQuantCols = 1024 * 4 * 8;  // widest row that is held in registers
+
 struct QuantArgs {
     const void* x;
     int8_t* codes;
@@ -307,7 +317,7 @@ struct QuantArgs {
     int type, cols;
 };
 
-template <int NV>
+template <int NV, int TYPE>
 __global__ void quantize_rows_kernel(const QuantArgs p, const int tpr) {
     __shared__ uint32_t slot[32];
     const long long row = static_cast<long long>(blockIdx.x) * (blockDim.x / tpr) + threadIdx.x / tpr;
@@ -319,7 +329,7 @@ __global__ void quantize_rows_kernel(const QuantArgs p, const int tpr) {
     for (int i = 0; i < NV; ++i) {
         const int c = (t + i * tpr) * 8;
         if (live && c < p.cols) {
-            unpack8(load_raw8(p.x, p.type, row * p.ld_x + c), p.type, v[i]);
+            unpack8(load_raw8(p.x, TYPE, row * p.ld_x + c), TYPE, v[i]);
 #pragma unroll
             for (int j = 0; j < 8; ++j) m = max(m, abs_bits(v[i][j]));
         }
@@ -440,6 +450,7 @@ __global__ void rope_qkv_any_kernel(const RopeArgs p) {
 // The same, sixteen elements per step: the two groups of eight whose pairs lie half the rotary part apart, or sixteen
 // neighbours (pairs side by side, elements behind the rotary part, values).  dim and rot are multiples of 16.  The
 // first step's loads are issued before the angles are computed.
+template <int XT, int OT>
 __global__ void rope_qkv_vec_kernel(const RopeArgs p) {
     __shared__ float2 cs[kRopeMaxDim / 2];
     const long long token = blockIdx.x;
@@ -456,22 +467,22 @@ __global__ void rope_qkv_vec_kernel(const RopeArgs p) {
     Raw8 r0, r1;
     if (u < units) {
         c = place(u, head, d0, d1);
-        r0 = load_raw8(p.x, p.x_type, token * p.ld_x + head * p.dim + d0);
-        r1 = load_raw8(p.x, p.x_type, token * p.ld_x + head * p.dim + d1);
+        r0 = load_raw8(p.x, XT, token * p.ld_x + head * p.dim + d0);
+        r1 = load_raw8(p.x, XT, token * p.ld_x + head * p.dim + d1);
     }
     const long long slot = rope_slot(p, token);
     rope_angles(p, token, cs);
     __syncthreads();
     while (u < units) {
         float a[8], b[8];
-        unpack8(r0, p.x_type, a);
-        unpack8(r1, p.x_type, b);
+        unpack8(r0, XT, a);
+        unpack8(r1, XT, b);
         const int head_now = head, d0_now = d0, d1_now = d1, c_now = c;
         u += blockDim.x;
         if (u < units) {
             c = place(u, head, d0, d1);
-            r0 = load_raw8(p.x, p.x_type, token * p.ld_x + head * p.dim + d0);
-            r1 = load_raw8(p.x, p.x_type, token * p.ld_x + head * p.dim + d1);
+            r0 = load_raw8(p.x, XT, token * p.ld_x + head * p.dim + d0);
+            r1 = load_raw8(p.x, XT, token * p.ld_x + head * p.dim + d1);
         }
         long long at;
         void* dst = rope_dest(p, token, slot, head_now, at);
@@ -506,8 +517,8 @@ __global__ void rope_qkv_vec_kernel(const RopeArgs p) {
                 }
             }
         }
-        store8(dst, p.out_type, at + d0_now, a);
-        store8(dst, p.out_type, at + d1_now, b);
+        store8(dst, OT, at + d0_now, a);
+        store8(dst, OT, at + d1_now, b);
     }
 }
 

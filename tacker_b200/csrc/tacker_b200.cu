@@ -1,7 +1,9 @@
 // libtacker_b200.so: the C-ABI entry points (see include/tacker_b200.h for the contract).
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <initializer_list>
+#include <type_traits>
 
 #include "host_launch.cuh"
 #include "more_kernels.cuh"
