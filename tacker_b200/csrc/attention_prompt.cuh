@@ -25,22 +25,9 @@
 #include <cuda.h>
 
 #include "attention_rows.cuh"
-#include "gemm_role2.cuh"
+#include "i8gemm.cuh"
 
 namespace tk {
-
-// one lane of a full warp, always the same
-__device__ __forceinline__ bool elect_lane() {
-    uint32_t e;
-    asm volatile(
-        "{\n"
-        ".reg .pred p;\n"
-        "elect.sync _|p, 0xffffffff;\n"
-        "selp.u32 %0, 1, 0, p;\n"
-        "}\n"
-        : "=r"(e));
-    return e != 0;
-}
 
 // The MMAs of a tile are issued back to back from one block of instructions: with N = 128 each takes 64 cycles of the
 // tensor pipe, and a loop that rebuilds its operands for each (138 cycles per MMA as measured) leaves the pipe idle.
@@ -146,30 +133,6 @@ __device__ __forceinline__ void fewer_registers() {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
 }
 
-// two fp32 operations per instruction
-__device__ __forceinline__ void fma2(float& x, float& y, float sx, float sy, float ax, float ay) {
-    asm("{\n"
-        ".reg .b64 v, w, c;\n"
-        "mov.b64 v, {%0, %1};\n"
-        "mov.b64 w, {%2, %3};\n"
-        "mov.b64 c, {%4, %5};\n"
-        "fma.rn.f32x2 v, v, w, c;\n"
-        "mov.b64 {%0, %1}, v;\n"
-        "}\n"
-        : "+f"(x), "+f"(y)
-        : "f"(sx), "f"(sy), "f"(ax), "f"(ay));
-}
-__device__ __forceinline__ void add2(float& x, float& y, float ax, float ay) {
-    asm("{\n"
-        ".reg .b64 v, w;\n"
-        "mov.b64 v, {%0, %1};\n"
-        "mov.b64 w, {%2, %3};\n"
-        "add.rn.f32x2 v, v, w;\n"
-        "mov.b64 {%0, %1}, v;\n"
-        "}\n"
-        : "+f"(x), "+f"(y)
-        : "f"(ax), "f"(ay));
-}
 // maxima that are NaN where an operand is
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float d;

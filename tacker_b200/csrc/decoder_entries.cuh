@@ -62,14 +62,14 @@ static int pow2_at_least(long long n, int lo, int hi) {
 
 constexpr long long kMaxGridX = 0x7fffffffll;
 
-// threads per row of the row kernels (two groups of eight columns each), threads and blocks of the launch
+// threads per row of the row kernels (sixteen columns each), threads and blocks of the launch
 struct RowShape {
     int tpr, block;
     long long blocks;
 };
 static RowShape row_shape(long long rows, int cols) {
     RowShape s;
-    s.tpr = pow2_at_least((cols / 8 + 1) / 2, 32, 1024);
+    s.tpr = pow2_at_least((cols + 15) / 16, 32, 1024);
     s.block = s.tpr < 128 ? 128 : s.tpr;
     const long long per = s.block / s.tpr;
     s.blocks = (rows + per - 1) / per;
@@ -130,6 +130,23 @@ static int launch_i8gemm(const void* A, long long lda, const void* B, long long 
     cfg.numAttrs = split > 1 ? 1 : 0;
     TK_CUDA(cudaLaunchKernelEx(&cfg, kernel, ta, tb, p, split, tiles_b));
     return TK_OK;
+}
+
+static int launch_i8gemm_pair(const void* A, long long lda, const void* B, long long ldb, const I8Args& p, DeviceInfo* d,
+                              cudaStream_t st) {
+    constexpr auto kernel = i8gemm_pair_kernel;
+    constexpr int smem = I8PairSmem::kBytes + 1024;
+    static_assert(smem <= kMaxDynSmem, "shared memory of a CTA");
+    int rc = enable_smem_once<kernel>(smem);
+    if (rc != TK_OK) return rc;
+    CUtensorMap ta, tb;
+    if ((rc = make_tmap_i8(&ta, A, p.M, p.K, lda, 128)) != TK_OK) return rc;
+    if ((rc = make_tmap_i8(&tb, B, p.N, p.K, ldb, 128)) != TK_OK) return rc;
+    const long long tiles = (p.M + 255ll) / 256 * ((p.N + 255ll) / 256);
+    if (tiles > kMaxGridX) return TK_ERR_SHAPE;
+    const long long pairs = std::min(tiles, static_cast<long long>(d->sm_count / 2));
+    kernel<<<static_cast<unsigned>(2 * pairs), 192, smem, st>>>(ta, tb, p);
+    return launch_error("i8gemm_pair_kernel launch");
 }
 
 // how many ranges of k: until the launch has a CTA for every SM, each range at least four stages long
@@ -258,7 +275,7 @@ TK_API int tk_norm_residual_rows(const void* a, int a_type, long long ld_a, int 
     p.post_gamma = post_gamma, p.post_beta = post_beta, p.pre_gamma = pre_gamma, p.pre_beta = pre_beta;
     p.gate = gate;
     p.ld_a = ld_a, p.ld_x = ld_x, p.ld_y = ld_y, p.ld_h = ld_h, p.ld_gate = ld_gate;
-    p.gate_rows = gate ? gate_rows : 1;
+    p.gate_rows = gate ? static_cast<uint32_t>(std::min(gate_rows, rows)) : 1u;
     p.rows = rows;
     p.a_type = a_type, p.x_type = x_type, p.h_type = h_type, p.cols = cols, p.post = post, p.layer = layer;
     p.scale = scale, p.eps = eps;
@@ -336,6 +353,8 @@ TK_API int tk_i8gemm(const void* A, long long lda, const float* scale_a, const v
     if (M <= 16) return launch_i8gemm<16, 5, true>(A, lda, B, ldb, p, i8_split(tn, kblocks, 2 * d->sm_count, 8), st);
     if (M <= 32) return launch_i8gemm<32, 5, true>(A, lda, B, ldb, p, i8_split(tn, kblocks, 2 * d->sm_count, 8), st);
     if (M <= 64) return launch_i8gemm<64, 4, true>(A, lda, B, ldb, p, i8_split(tn, kblocks, 2 * d->sm_count, 8), st);
+    // Large products on CTA pairs: when their 256 x 256 tiles give every pair of SMs something to do
+    if ((M + 255ll) / 256 * ((N + 255ll) / 256) >= d->sm_count / 2) return launch_i8gemm_pair(A, lda, B, ldb, p, d, st);
     const long long tm = (M + 127) / 128;
     return launch_i8gemm<128, 3, false>(A, lda, B, ldb, p, i8_split(tm * tn, kblocks, 2 * d->sm_count, 8), st);
 }

@@ -6,10 +6,23 @@
 // Operand tiles are 128 bytes (128 values of k) wide, K-major, 128-byte swizzled by TMA; rows and k beyond the matrices
 // arrive as zeros and add nothing, so no size has to be a multiple of a tile.
 #pragma once
-#include "gemm_role2.cuh"
+#include "kernels.cuh"
 #include "row_ops.cuh"
 
 namespace tk {
+
+// one lane of a full warp, always the same
+__device__ __forceinline__ bool elect_lane() {
+    uint32_t e;
+    asm volatile(
+        "{\n"
+        ".reg .pred p;\n"
+        "elect.sync _|p, 0xffffffff;\n"
+        "selp.u32 %0, 1, 0, p;\n"
+        "}\n"
+        : "=r"(e));
+    return e != 0;
+}
 
 struct I8Args {
     const float* scale_a;  // [M]
@@ -45,14 +58,60 @@ __host__ __device__ constexpr uint32_t umma_idesc_i8_s32(uint32_t m, uint32_t n)
 
 constexpr int kI8BK = 128;  // bytes of k per stage
 
+// ---- output ----------------------------------------------------------------------------------------------------
+constexpr int kI8OutPitch = 36;                       // floats per staged row: conflict-free by rows and by columns
+constexpr int kI8OutBytes = 32 * kI8OutPitch * 4;     // one warp's staging
+
+// 32 x 32 sums of a warp (one row per lane) on their way to out rows row0 .., columns col0 ..: times the row's scale into
+// shared memory, then times the column's scale and stored with neighbouring lanes on neighbouring columns.  A row per lane
+// and store would touch 32 lines with every instruction.
+__device__ __forceinline__ void i8_store_chunk(const I8Args& p, float* stage, const uint32_t (&v)[32], float row_scale,
+                                               int row0, int col0, int lane) {
+    float4* mine = reinterpret_cast<float4*>(stage + lane * kI8OutPitch);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        mine[i] = make_float4(static_cast<float>(static_cast<int>(v[4 * i])) * row_scale,
+                              static_cast<float>(static_cast<int>(v[4 * i + 1])) * row_scale,
+                              static_cast<float>(static_cast<int>(v[4 * i + 2])) * row_scale,
+                              static_cast<float>(static_cast<int>(v[4 * i + 3])) * row_scale);
+    __syncwarp();
+    if (p.vec && col0 + 32 <= p.N) {
+        // eight columns per lane: four lanes per row, eight rows at a time
+        const int c = col0 + (lane & 3) * 8;
+        float sc[8], b[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sc[i] = __ldg(p.scale_b + c + i);
+        if (p.bias) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) b[i] = __ldg(p.bias + c + i);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int r = 8 * i + (lane >> 2);
+            const float4* src = reinterpret_cast<const float4*>(stage + r * kI8OutPitch + (lane & 3) * 8);
+            const float4 x = src[0], y = src[1];
+            const float o[8] = {x.x * sc[0] + b[0], x.y * sc[1] + b[1], x.z * sc[2] + b[2], x.w * sc[3] + b[3],
+                                y.x * sc[4] + b[4], y.y * sc[5] + b[5], y.z * sc[6] + b[6], y.w * sc[7] + b[7]};
+            if (row0 + r < p.M) store8(p.out, p.out_type, (row0 + r) * p.ld_out + c, o);
+        }
+    } else if (col0 + lane < p.N) {
+        const int c = col0 + lane;
+        const float sc = __ldg(p.scale_b + c), b = p.bias ? __ldg(p.bias + c) : 0.0f;
+        const int n = min(32, p.M - row0);
+        for (int r = 0; r < n; ++r) store1(p.out, p.out_type, (row0 + r) * p.ld_out + c, stage[r * kI8OutPitch + lane] * sc + b);
+    }
+    __syncwarp();
+}
+
 template <int BN, int STAGES>
 struct I8Smem {
     static constexpr int kABytes = 128 * kI8BK;
     static constexpr int kBBytes = BN * kI8BK;
     static constexpr int kStageBytes = kABytes + kBBytes;
-    static constexpr int kPartBytes = 128 * BN * 4;  // partial sums of a K range, over the drained stages
+    static constexpr int kPartBytes = 128 * (BN + 1) * 4;  // partial sums of a range of k, over the drained stages
     static constexpr int kRing = STAGES * kStageBytes;
-    static constexpr int kBarOffset = kRing > kPartBytes ? kRing : kPartBytes;
+    static constexpr int kBarOffset = ((kRing > kPartBytes ? kRing : kPartBytes) + 7) / 8 * 8;
+    static_assert(4 * kI8OutBytes <= kRing, "the output warps' staging fits over the drained stages");
     static constexpr int kTmemSlotOffset = kBarOffset + (2 * STAGES + 1) * 8;
     static constexpr int kAbortOffset = kTmemSlotOffset + 4;
     static constexpr int kBytes = kAbortOffset + 4;
@@ -162,7 +221,9 @@ i8gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant_
     const uint32_t t_lane = tmem + (static_cast<uint32_t>(q * 32) << 16);
     const int r = row_a + q * 32 + lane;  // this thread's row of the MMA
     if (split > 1) {
-        int* part = reinterpret_cast<int*>(smem);  // [BN][128]
+        // the partial sums lie in shared memory so that the lanes that finish them read and store neighbours: with SWAP an
+        // output row runs along the rows of the MMA, otherwise along its columns
+        int* part = reinterpret_cast<int*>(smem);
         if (warp >= 2 && good) {
 #pragma unroll 1
             for (int c = 0; c < BN; c += 32) {
@@ -171,65 +232,75 @@ i8gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant_
                 tmem_ld_wait();
 #pragma unroll
                 for (int j = 0; j < 32; ++j)
-                    if (c + j < BN) part[(c + j) * 128 + q * 32 + lane] = static_cast<int>(v[j]);
+                    if (c + j < BN) part[SWAP ? (c + j) * 128 + q * 32 + lane : (q * 32 + lane) * (BN + 1) + c + j] = static_cast<int>(v[j]);
             }
         }
         __syncwarp();
         cluster_arrive();
         cluster_wait();
         if (warp >= 2 && good) {
-            const int share = BN / split, c0 = rank * share;
-            const int rows = SWAP ? p.N : p.M, cols = SWAP ? p.M : p.N;
-            const float sr = r < rows ? (SWAP ? p.scale_b[r] : p.scale_a[r]) : 0.0f;
-            const float bias_r = SWAP && p.bias && r < rows ? p.bias[r] : 0.0f;
-            const uint32_t mine = smem_base + 4u * (q * 32 + lane);
+            if (SWAP) {
+                const float sr = r < p.N ? p.scale_b[r] : 0.0f, b = p.bias && r < p.N ? p.bias[r] : 0.0f;
+                const int share = BN / split;
 #pragma unroll 4
-            for (int c = c0; c < c0 + share; ++c) {
-                const int cg = row_b + c;
-                if (cg >= cols) break;
-                int sum = 0;
-                for (int s = 0; s < split; ++s) sum += ld_shared_cluster_s32(mapa_shared(mine + 512u * c, s));
-                const float sc = SWAP ? p.scale_a[cg] : p.scale_b[cg];
-                float v = static_cast<float>(sum) * (SWAP ? sc : sr) * (SWAP ? sr : sc);
-                v += SWAP ? bias_r : (p.bias ? p.bias[cg] : 0.0f);
-                if (r < rows)
-                    store1(p.out, p.out_type, SWAP ? cg * p.ld_out + r : r * p.ld_out + cg, v);
+                for (int c = rank * share; c < (rank + 1) * share; ++c) {
+                    const int token = row_b + c;
+                    if (token >= p.M) break;
+                    int sum = 0;
+                    for (int s = 0; s < split; ++s)
+                        sum += ld_shared_cluster_s32(mapa_shared(smem_base + 4u * (c * 128 + q * 32 + lane), s));
+                    if (r < p.N)
+                        store1(p.out, p.out_type, token * p.ld_out + r, static_cast<float>(sum) * p.scale_a[token] * sr + b);
+                }
+            } else {
+                const int share = 128 / split;
+                for (int i = rank * share + q; i < (rank + 1) * share; i += 4) {
+                    const int token = row_a + i;
+                    if (token >= p.M) break;
+                    const float sa = p.scale_a[token];
+#pragma unroll
+                    for (int c = lane; c < BN; c += 32) {
+                        const int col = row_b + c;
+                        if (col >= p.N) break;
+                        int sum = 0;
+                        for (int s = 0; s < split; ++s)
+                            sum += ld_shared_cluster_s32(mapa_shared(smem_base + 4u * (i * (BN + 1) + c), s));
+                        store1(p.out, p.out_type, token * p.ld_out + col,
+                               static_cast<float>(sum) * sa * __ldg(p.scale_b + col) + (p.bias ? __ldg(p.bias + col) : 0.0f));
+                    }
+                }
             }
         }
         __syncwarp();
         cluster_arrive();  // no CTA leaves while another may still read its partial sums
         cluster_wait();
     } else if (warp >= 2 && good) {
-        const int rows = SWAP ? p.N : p.M, cols = SWAP ? p.M : p.N;
-        const float sr = r < rows ? (SWAP ? p.scale_b[r] : p.scale_a[r]) : 0.0f;
-        const float bias_r = SWAP && p.bias && r < rows ? p.bias[r] : 0.0f;
+        if (SWAP) {
+            const float sr = r < p.N ? p.scale_b[r] : 0.0f, b = p.bias && r < p.N ? p.bias[r] : 0.0f;
 #pragma unroll 1
-        for (int c = 0; c < BN; c += 32) {
-            if (row_b + c >= cols) break;
-            uint32_t v[32];
-            __syncwarp();
-            tmem_ld_32x32(t_lane + c, v);
-            tmem_ld_wait();
+            for (int c = 0; c < BN && row_b + c < p.M; c += 32) {
+                uint32_t v[32];
+                __syncwarp();
+                tmem_ld_32x32(t_lane + c, v);
+                tmem_ld_wait();
 #pragma unroll
-            for (int j = 0; j < 32; j += 8) {
-                const int cg = row_b + c + j;
-                if (r >= rows || c + j >= BN || cg >= cols) break;
-                float o[8];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const int ci = min(cg + i, cols - 1);
-                    const float sc = __ldg((SWAP ? p.scale_a : p.scale_b) + ci);
-                    o[i] = static_cast<float>(static_cast<int>(v[j + i])) * (SWAP ? sc : sr) * (SWAP ? sr : sc);
-                    o[i] += SWAP ? bias_r : (p.bias ? __ldg(p.bias + ci) : 0.0f);
+                for (int j = 0; j < 32; ++j) {
+                    const int token = row_b + c + j;
+                    if (c + j >= BN || token >= p.M) break;
+                    if (r < p.N)
+                        store1(p.out, p.out_type, token * p.ld_out + r,
+                               static_cast<float>(static_cast<int>(v[j])) * p.scale_a[token] * sr + b);
                 }
-                if (!SWAP && p.vec && cg + 8 <= cols) {
-                    store8(p.out, p.out_type, r * p.ld_out + cg, o);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        if (cg + i < cols)
-                            store1(p.out, p.out_type, SWAP ? (cg + i) * p.ld_out + r : r * p.ld_out + cg + i, o[i]);
-                }
+            }
+        } else {
+            const float sa = r < p.M ? p.scale_a[r] : 0.0f;
+#pragma unroll 1
+            for (int c = 0; c < BN && row_b + c < p.N; c += 32) {
+                uint32_t v[32];
+                __syncwarp();
+                tmem_ld_32x32(t_lane + c, v);
+                tmem_ld_wait();
+                i8_store_chunk(p, reinterpret_cast<float*>(smem + q * kI8OutBytes), v, sa, row_a + q * 32, row_b + c, lane);
             }
         }
     }
@@ -239,6 +310,217 @@ i8gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant_
     __syncthreads();
     tc_fence_after_sync();
     if (warp == 1) tmem_dealloc(tmem, kTmemCols);
+}
+
+// ---- the product on CTA pairs ------------------------------------------------------------------------------------
+// Large products: 256 x 256 tiles on clusters of two CTAs (tcgen05.mma.cta_group::2), one persistent pair per two SMs.  Each
+// CTA loads its own 128 rows of A and one half of the tile's rows of B, so that a stage of 128 k costs it 32 KB for 128 x 256
+// results instead of the 48 KB of a tile of its own: at 512 cycles a stage, 64 bytes a cycle from L2.  The roles and signals
+// are those of the fp16 role (gemm_role2.cuh): full barriers in the leader, empty barriers in both CTAs, two accumulators of
+// 256 columns so that a tile is written while the next one is summed.
+__device__ __forceinline__ void umma_i8_pair_x4(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                                uint32_t accumulate) {
+    asm volatile(
+        "{\n"
+        ".reg .pred p, t;\n"
+        ".reg .b64 a, b;\n"
+        "setp.ne.b32 p, %4, 0;\n"
+        "setp.eq.b32 t, 0, 0;\n"
+        "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n"
+        "add.s64 a, %1, 2;\n"
+        "add.s64 b, %2, 2;\n"
+        "tcgen05.mma.cta_group::2.kind::i8 [%0], a, b, %3, t;\n"
+        "add.s64 a, %1, 4;\n"
+        "add.s64 b, %2, 4;\n"
+        "tcgen05.mma.cta_group::2.kind::i8 [%0], a, b, %3, t;\n"
+        "add.s64 a, %1, 6;\n"
+        "add.s64 b, %2, 6;\n"
+        "tcgen05.mma.cta_group::2.kind::i8 [%0], a, b, %3, t;\n"
+        "}\n" ::"r"(d_tmem),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void tma_load_2d_pair(uint32_t dst_smem, const void* tmap, uint32_t bar_cluster_addr, int x, int y) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+        ::"r"(dst_smem), "l"(reinterpret_cast<uint64_t>(tmap)), "r"(bar_cluster_addr), "r"(x), "r"(y)
+        : "memory");
+}
+
+struct I8PairSmem {
+    static constexpr int kStages = 6;
+    static constexpr int kTileBytes = 128 * kI8BK;
+    static constexpr int kStageBytes = 2 * kTileBytes;
+    static constexpr int kOutOffset = kStages * kStageBytes;
+    static constexpr int kBarOffset = kOutOffset + 4 * kI8OutBytes;
+    static constexpr int kNumBars = 2 * kStages + 4;
+    static constexpr int kTmemSlotOffset = kBarOffset + kNumBars * 8;
+    static constexpr int kAbortOffset = kTmemSlotOffset + 4;
+    static constexpr int kBytes = kAbortOffset + 4;
+};
+
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1)
+i8gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b, const I8Args p) {
+    using L = I8PairSmem;
+    constexpr int ST = L::kStages;
+    constexpr uint32_t kIdesc = umma_idesc_i8_s32(256, 256);
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = align_smem_1024(smem_raw);
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_ctarank();
+    const bool leader_cta = rank == 0;
+    const uint32_t base = smem_u32(smem), bars = base + L::kBarOffset;
+    auto full_bar = [&](int s) { return bars + 8u * s; };
+    auto empty_bar = [&](int s) { return bars + 8u * (ST + s); };
+    auto tfull_bar = [&](int a) { return bars + 8u * (2 * ST + a); };
+    auto tempty_bar = [&](int a) { return bars + 8u * (2 * ST + 2 + a); };
+    volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + L::kTmemSlotOffset);
+    volatile uint32_t* abort_flag = reinterpret_cast<volatile uint32_t*>(smem + L::kAbortOffset);
+    const int pair = blockIdx.x >> 1, npairs = gridDim.x >> 1;
+    const int tiles_m = (p.M + 255) / 256, tiles_n = (p.N + 255) / 256, kblocks = (p.K + kI8BK - 1) / kI8BK;
+    // at most 2^31 / 2^16 x 2^31 / 2^16 tiles: the launcher keeps the count below 2^31
+    const int tiles = tiles_m * tiles_n;
+
+    if (warp == 0 && lane == 0) {
+        *abort_flag = 0u;
+        for (int s = 0; s < ST; ++s) {
+            mbar_init(full_bar(s), 1);   // used in the leader only
+            mbar_init(empty_bar(s), 1);
+        }
+        for (int a = 0; a < 2; ++a) {
+            mbar_init(tfull_bar(a), 1);
+            mbar_init(tempty_bar(a), 8);  // used in the leader only: four output warps of each CTA
+        }
+        fence_mbar_init();
+        tma_prefetch_desc(&tmap_a);
+        tma_prefetch_desc(&tmap_b);
+    }
+    __syncwarp();
+    cluster_arrive();  // publishes the barrier initialisation to the peer
+    cluster_wait();
+    if (warp == 1) {
+        tmem_alloc_pair(smem_u32(const_cast<uint32_t*>(tmem_slot)), 512);
+        tmem_relinquish_pair();
+    }
+    tc_fence_before_sync();
+    __syncthreads();
+    tc_fence_after_sync();
+    const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
+
+    if (warp == 0) {
+        // ---------------- TMA producer (both CTAs) ----------------
+        if (lane == 0) {
+            int stage = 0, waits = 0;
+            uint32_t phase = 0;
+            bool ok = true;
+            const uint32_t empty_peer0 = mapa_shared(empty_bar(0), 1u);
+            // wait number i of the leader sees the commit of K-block i - ST; every one after the first ST, which pass without
+            // an arrival in both CTAs, is passed on to the peer
+            auto wait_empty = [&]() {
+                ok = mbar_wait(empty_bar(stage), phase ^ 1u, abort_flag, p.status, DEV_TIMEOUT_EMPTY);
+                if (ok && leader_cta && waits >= ST) mbar_arrive_cluster_relaxed(empty_peer0 + 8u * stage);
+                ++waits;
+                return ok;
+            };
+            auto advance = [&]() {
+                if (++stage == ST) {
+                    stage = 0;
+                    phase ^= 1u;
+                }
+            };
+            for (int tile = pair; ok && tile < tiles; tile += npairs) {
+                const int row_a = tile % tiles_m * 256 + static_cast<int>(rank) * 128;
+                const int row_b = tile / tiles_m * 256 + static_cast<int>(rank) * 128;
+                for (int kb = 0; kb < kblocks; ++kb) {
+                    if (!wait_empty()) break;
+                    if (leader_cta) mbar_arrive_expect_tx(full_bar(stage), 2u * L::kStageBytes);
+                    const uint32_t full_leader = mapa_shared(full_bar(stage), 0u);
+                    const uint32_t dst = base + stage * L::kStageBytes;
+                    tma_load_2d_pair(dst, &tmap_a, full_leader, kb * kI8BK, row_a);
+                    tma_load_2d_pair(dst + L::kTileBytes, &tmap_b, full_leader, kb * kI8BK, row_b);
+                    advance();
+                }
+            }
+            // the last commits arrive on the empty barriers asynchronously: no CTA retires before they have landed
+            for (int s = 0; s < ST && ok; ++s) {
+                wait_empty();
+                advance();
+            }
+        }
+    } else if (warp == 1) {
+        // ---------------- MMA issuer (leader only) ----------------
+        if (leader_cta) {
+            const bool issuer = elect_lane();
+            int stage = 0;
+            uint32_t phase = 0, it = 0;
+            bool ok = true;
+            auto wait = [&](uint32_t bar, uint32_t parity, unsigned code) {
+                return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, p.status, code)) != 0;
+            };
+            for (int tile = pair; ok && tile < tiles; tile += npairs, ++it) {
+                const uint32_t as = it & 1u;
+                ok = wait(tempty_bar(as), ((it >> 1) & 1u) ^ 1u, DEV_TIMEOUT_TMEM_EMPTY);
+                if (!ok) break;
+                tc_fence_after_sync();
+                for (int kb = 0; kb < kblocks; ++kb) {
+                    ok = wait(full_bar(stage), phase, DEV_TIMEOUT_FULL);
+                    if (!ok) break;
+                    tc_fence_after_sync();
+                    const uint32_t src = base + stage * L::kStageBytes;
+                    const uint64_t a_desc = umma_smem_desc_sw128(src), b_desc = umma_smem_desc_sw128(src + L::kTileBytes);
+                    if (issuer) {
+                        umma_i8_pair_x4(tmem + as * 256, a_desc, b_desc, kIdesc, kb != 0);
+                        umma_commit_pair(empty_bar(stage));
+                    }
+                    __syncwarp();
+                    if (++stage == ST) {
+                        stage = 0;
+                        phase ^= 1u;
+                    }
+                }
+                if (ok && issuer) {
+                    umma_commit_pair(tfull_bar(as));
+                    umma_commit_pair(mapa_shared(tfull_bar(as), 1u));
+                }
+                __syncwarp();
+            }
+            // the peer's output warps arrive on this CTA's barriers: wait until both accumulators have been given back
+            for (int j = 0; j < 2 && ok; ++j, ++it)
+                ok = wait(tempty_bar(it & 1u), ((it >> 1) & 1u) ^ 1u, DEV_TIMEOUT_TMEM_EMPTY);
+        }
+    } else {
+        // ---------------- output (both CTAs) ----------------
+        const int q = warp & 3;
+        const uint32_t tempty_leader0 = mapa_shared(tempty_bar(0), 0u);
+        float* stage = reinterpret_cast<float*>(smem + L::kOutOffset + q * kI8OutBytes);
+        uint32_t it = 0;
+        bool ok = true;
+        for (int tile = pair; ok && tile < tiles; tile += npairs, ++it) {
+            const uint32_t as = it & 1u;
+            ok = __all_sync(0xffffffffu, mbar_wait(tfull_bar(as), (it >> 1) & 1u, abort_flag, p.status, DEV_TIMEOUT_TMEM_FULL)) != 0;
+            if (!ok) break;
+            tc_fence_after_sync();
+            const int row0 = tile % tiles_m * 256 + static_cast<int>(rank) * 128 + q * 32, col0 = tile / tiles_m * 256;
+            const float sa = row0 + lane < p.M ? __ldg(p.scale_a + row0 + lane) : 0.0f;
+            const uint32_t t_lane = tmem + (static_cast<uint32_t>(q * 32) << 16) + as * 256;
+#pragma unroll 1
+            for (int c = 0; c < 256 && col0 + c < p.N && row0 < p.M; c += 32) {
+                uint32_t v[32];
+                tmem_ld_32x32(t_lane + c, v);
+                tmem_ld_wait();
+                i8_store_chunk(p, stage, v, sa, row0, col0 + c, lane);
+            }
+            tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster_relaxed(tempty_leader0 + 8u * as);
+        }
+    }
+    __syncwarp();
+    if (*abort_flag) __nanosleep(1000000u);  // let bulk copies still in flight land before shared memory is released
+    tc_fence_before_sync();
+    __syncthreads();
+    tc_fence_after_sync();
+    if (warp == 1) tmem_dealloc_pair(tmem, 512);
 }
 
 }  // namespace tk

@@ -87,6 +87,42 @@ __device__ __forceinline__ void load8f(const float* p, int i, float (&v)[8]) {
     v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
 }
 
+// two fp32 operations per instruction
+__device__ __forceinline__ void fma2(float& x, float& y, float sx, float sy, float ax, float ay) {
+    asm("{\n"
+        ".reg .b64 v, w, c;\n"
+        "mov.b64 v, {%0, %1};\n"
+        "mov.b64 w, {%2, %3};\n"
+        "mov.b64 c, {%4, %5};\n"
+        "fma.rn.f32x2 v, v, w, c;\n"
+        "mov.b64 {%0, %1}, v;\n"
+        "}\n"
+        : "+f"(x), "+f"(y)
+        : "f"(sx), "f"(sy), "f"(ax), "f"(ay));
+}
+__device__ __forceinline__ void add2(float& x, float& y, float ax, float ay) {
+    asm("{\n"
+        ".reg .b64 v, w;\n"
+        "mov.b64 v, {%0, %1};\n"
+        "mov.b64 w, {%2, %3};\n"
+        "add.rn.f32x2 v, v, w;\n"
+        "mov.b64 {%0, %1}, v;\n"
+        "}\n"
+        : "+f"(x), "+f"(y)
+        : "f"(ax), "f"(ay));
+}
+__device__ __forceinline__ void mul2(float& x, float& y, float sx, float sy) {
+    asm("{\n"
+        ".reg .b64 v, w;\n"
+        "mov.b64 v, {%0, %1};\n"
+        "mov.b64 w, {%2, %3};\n"
+        "mul.rn.f32x2 v, v, w;\n"
+        "mov.b64 {%0, %1}, v;\n"
+        "}\n"
+        : "+f"(x), "+f"(y)
+        : "f"(sx), "f"(sy));
+}
+
 // Sum over the `tpr` threads of a row (a power of two, at least a warp).  `slots` is a shared array of 2 x 32 floats, used in
 // turn so that one barrier per sum is enough; `turn` counts the sums.  Every thread of the block calls it, the same number
 // of times.
@@ -94,7 +130,7 @@ __device__ __forceinline__ float row_sum(float v, int tpr, float* slots, int& tu
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     if (tpr == 32) return v;
-    const int warp = threadIdx.x >> 5, per = tpr >> 5, first = warp / per * per, lane = threadIdx.x & 31;
+    const int warp = threadIdx.x >> 5, per = tpr >> 5, first = warp & -per, lane = threadIdx.x & 31;  // powers of two
     float* slot = slots + 32 * (turn++ & 1);
     if (lane == 0) slot[warp] = v;
     __syncthreads();
@@ -120,110 +156,133 @@ struct NormArgs {
     const float* pre_gamma;
     const float* pre_beta;
     const float* gate;  // rows r of a share gate row r / gate_rows; null = 1
-    long long ld_a, ld_x, ld_y, ld_h, ld_gate, gate_rows, rows;
+    long long ld_a, ld_x, ld_y, ld_h, ld_gate, rows;
+    uint32_t gate_rows;  // 32 bits: a 64-bit division is a hundred instructions per thread and row
     int a_type, x_type, h_type, cols, post, layer;
     float scale, eps;
 };
 
 // One row per `tpr` threads, two groups of eight columns per thread in registers; the blocks stay and walk over the rows,
-// with the next row's a and x on their way while this one is summed up.  The types are compile-time constants: chosen
-// at run time, the conversions alone were two thirds of 54 instructions per element and the kernel was bound by issue
-// (80 us at 8191 x 4096 bf16 instead of 48, of which memory needs 41).
+// with the next row's a and x on their way while this one is summed up.  The types are compile-time constants: chosen at
+// run time, the conversions were most of 54 instructions per element.  Groups of four columns, whose fp32 weights would
+// come without gaps between the lanes, were slower (66 us against 58 at 8191 x 4096 bf16: more accesses).
 constexpr int kNormCols = 1024 * 2 * 8;  // widest row
 template <int AT, int XT, int HT>
 __global__ void __launch_bounds__(1024) norm_residual_kernel(const NormArgs p, const int tpr) {
     __shared__ float slots[64];
-    const int per_block = blockDim.x / tpr, t = threadIdx.x & (tpr - 1);
-    const long long step = static_cast<long long>(gridDim.x) * per_block;
+    const int t = threadIdx.x & (tpr - 1), c0 = t * 8, c1 = (t + tpr) * 8;
+    const uint32_t rows = static_cast<uint32_t>(p.rows), per_block = blockDim.x >> (31 - __clz(tpr));
+    const uint32_t step = gridDim.x * per_block;
+    const bool in0 = c0 < p.cols, in1 = c1 < p.cols;
     const float inv_cols = 1.0f / static_cast<float>(p.cols);
     int turn = 0;
-    Raw8 ar[2], xr[2];
-    auto fetch = [&](const void* src, int type, long long ld, long long row, Raw8 (&r)[2]) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int c = (t + i * tpr) * 8;
-            if (src && row < p.rows && c < p.cols) r[i] = load_raw8(src, type, row * ld + c);
-        }
-    };
-    long long row = static_cast<long long>(blockIdx.x) * per_block + threadIdx.x / tpr;
-    fetch(p.a, AT, p.ld_a, row, ar);
-    fetch(p.x, XT, p.ld_x, row, xr);
+    Raw8 a0, a1, x0, x1;
+    uint32_t row = blockIdx.x * per_block + (threadIdx.x >> (31 - __clz(tpr)));
+    // this thread's first group of the row at hand in each array
+    long long at_a = row * p.ld_a + c0, at_x = row * p.ld_x + c0, at_y = row * p.ld_y + c0, at_h = row * p.ld_h + c0;
+    const int apart = tpr * 8;
+    const bool has_x = p.x != nullptr;
+    if (row < rows && in0) a0 = load_raw8(p.a, AT, at_a);
+    if (row < rows && in1) a1 = load_raw8(p.a, AT, at_a + apart);
+    if (has_x && row < rows && in0) x0 = load_raw8(p.x, XT, at_x);
+    if (has_x && row < rows && in1) x1 = load_raw8(p.x, XT, at_x + apart);
     // all threads of a block make the same number of rounds, for the barriers in the sums
-    for (long long base = static_cast<long long>(blockIdx.x) * per_block; base < p.rows; base += step, row += step) {
-        const bool live = row < p.rows;
-        float v[2][8];
+    for (uint32_t base = blockIdx.x * per_block; base < rows; base += step) {
+        const bool live0 = row < rows && in0, live1 = row < rows && in1;
+        const uint32_t next = row + step;
+        float v[8], w[8];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[i][j] = 0.0f;
-            if (live && (t + i * tpr) * 8 < p.cols) unpack8(ar[i], AT, v[i]);
-        }
-        fetch(p.a, AT, p.ld_a, row + step, ar);
-        // v <- (v - mean) * rstd over the columns of the row; the padding columns stay out of the sums
+        for (int j = 0; j < 8; ++j) v[j] = w[j] = 0.0f;
+        if (live0) unpack8(a0, AT, v);
+        if (live1) unpack8(a1, AT, w);
+        at_a += step * p.ld_a;
+        if (next < rows && in0) a0 = load_raw8(p.a, AT, at_a);
+        if (next < rows && in1) a1 = load_raw8(p.a, AT, at_a + apart);
+        // (v, w) <- ((v, w) - mean) * rstd over the columns of the row; groups that do not exist stay zero
         auto normalise = [&]() {
-            float mean = 0.0f;
             if (p.layer) {
-                float s = 0.0f;
+                float s0 = 0.0f, s1 = 0.0f;
 #pragma unroll
-                for (int i = 0; i < 2; ++i)
+                for (int j = 0; j < 8; j += 2) add2(s0, s1, v[j], v[j + 1]), add2(s0, s1, w[j], w[j + 1]);
+                const float mean = row_sum(s0 + s1, tpr, slots, turn) * inv_cols;
+                const float m0 = in0 ? -mean : 0.0f, m1 = in1 ? -mean : 0.0f;
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) s += v[i][j];
-                mean = row_sum(s, tpr, slots, turn) * inv_cols;
+                for (int j = 0; j < 8; j += 2) add2(v[j], v[j + 1], m0, m0), add2(w[j], w[j + 1], m1, m1);
             }
-            float q = 0.0f;
+            float q0 = 0.0f, q1 = 0.0f, r0 = 0.0f, r1 = 0.0f;
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                if ((t + i * tpr) * 8 < p.cols) {
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        v[i][j] -= mean;
-                        q = fmaf(v[i][j], v[i][j], q);
-                    }
-                }
+            for (int j = 0; j < 8; j += 2) {
+                float sx = v[j], sy = v[j + 1], ux = w[j], uy = w[j + 1];
+                fma2(sx, sy, sx, sy, q0, q1);
+                fma2(ux, uy, ux, uy, r0, r1);
+                q0 = sx, q1 = sy, r0 = ux, r1 = uy;
             }
-            const float rstd = rsqrtf(row_sum(q, tpr, slots, turn) * inv_cols + p.eps);
+            const float rstd = rsqrtf(row_sum((q0 + q1) + (r0 + r1), tpr, slots, turn) * inv_cols + p.eps);
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-                for (int j = 0; j < 8; ++j) v[i][j] *= rstd;
+            for (int j = 0; j < 8; j += 2) mul2(v[j], v[j + 1], rstd, rstd), mul2(w[j], w[j + 1], rstd, rstd);
         };
-        auto affine = [&](const float* gamma, const float* beta, int i, int c) {
-            float g[8];
-            if (gamma) {
-                load8f(gamma, c, g);
+        auto times = [&](const float* g) {
+            float u[8];
+            if (live0) {
+                load8f(g, c0, u);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) v[i][j] *= g[j];
+                for (int j = 0; j < 8; j += 2) mul2(v[j], v[j + 1], u[j], u[j + 1]);
             }
-            if (beta) {
-                load8f(beta, c, g);
+            if (live1) {
+                load8f(g, c1, u);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) v[i][j] += g[j];
+                for (int j = 0; j < 8; j += 2) mul2(w[j], w[j + 1], u[j], u[j + 1]);
             }
         };
-        if (p.post) normalise();
-        const float* gate = p.gate && live ? p.gate + row / p.gate_rows * p.ld_gate : nullptr;
+        auto plus = [&](const float* g) {
+            float u[8];
+            if (live0) {
+                load8f(g, c0, u);
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int c = (t + i * tpr) * 8;
-            if (!live || c >= p.cols) continue;
-            if (p.post) affine(p.post_gamma, p.post_beta, i, c);
-            if (gate) affine(gate, nullptr, i, c);
-            float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-            if (p.x) unpack8(xr[i], XT, x);
+                for (int j = 0; j < 8; j += 2) add2(v[j], v[j + 1], u[j], u[j + 1]);
+            }
+            if (live1) {
+                load8f(g, c1, u);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[i][j] = fmaf(p.scale, v[i][j], x[j]);
-            if (p.y) store8(p.y, XT, row * p.ld_y + c, v[i]);
+                for (int j = 0; j < 8; j += 2) add2(w[j], w[j + 1], u[j], u[j + 1]);
+            }
+        };
+        if (p.post) {
+            normalise();
+            if (p.post_gamma) times(p.post_gamma);
+            if (p.post_beta) plus(p.post_beta);
         }
-        fetch(p.x, XT, p.ld_x, row + step, xr);
-        if (!p.h) continue;
-        normalise();
+        if (p.gate) times(p.gate + (row < rows ? row / p.gate_rows * p.ld_gate : 0));
+        {
+            float x[8];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int c = (t + i * tpr) * 8;
-            if (!live || c >= p.cols) continue;
-            affine(p.pre_gamma, p.pre_beta, i, c);
-            store8(p.h, HT, row * p.ld_h + c, v[i]);
+            for (int j = 0; j < 8; ++j) x[j] = 0.0f;
+            if (has_x && live0) unpack8(x0, XT, x);
+#pragma unroll
+            for (int j = 0; j < 8; j += 2) fma2(v[j], v[j + 1], p.scale, p.scale, x[j], x[j + 1]);
+            if (has_x && live1) unpack8(x1, XT, x);
+#pragma unroll
+            for (int j = 0; j < 8; j += 2) fma2(w[j], w[j + 1], p.scale, p.scale, x[j], x[j + 1]);
+            if (!in1) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) w[j] = 0.0f;  // x of the first group went into one that does not exist
+            }
         }
+        if (p.y && live0) store8(p.y, XT, at_y, v);
+        if (p.y && live1) store8(p.y, XT, at_y + apart, w);
+        at_x += step * p.ld_x;
+        if (has_x && next < rows && in0) x0 = load_raw8(p.x, XT, at_x);
+        if (has_x && next < rows && in1) x1 = load_raw8(p.x, XT, at_x + apart);
+        if (p.h) {
+            normalise();
+            if (p.pre_gamma) times(p.pre_gamma);
+            if (p.pre_beta) plus(p.pre_beta);
+            if (live0) store8(p.h, HT, at_h, v);
+            if (live1) store8(p.h, HT, at_h + apart, w);
+        }
+        row = next;
+        at_y += step * p.ld_y;
+        at_h += step * p.ld_h;
     }
 }
 
@@ -235,7 +294,7 @@ __global__ void norm_residual_any_kernel(const NormArgs p) {
     const int tpr = blockDim.x;
     const long long row = blockIdx.x;
     const float inv_cols = 1.0f / static_cast<float>(p.cols);
-    const float* gate = p.gate ? p.gate + row / p.gate_rows * p.ld_gate : nullptr;
+    const float* gate = p.gate ? p.gate + static_cast<uint32_t>(row) / p.gate_rows * p.ld_gate : nullptr;
     auto stats = [&](auto value, float& mean, float& rstd) {
         mean = 0.0f;
         if (p.layer) {
@@ -301,7 +360,7 @@ __device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x
 __device__ __forceinline__ uint32_t row_umax(uint32_t v, int tpr, uint32_t* slot) {
     v = __reduce_max_sync(0xffffffffu, v);
     if (tpr == 32) return v;
-    const int warp = threadIdx.x >> 5, per = tpr >> 5, first = warp / per * per, lane = threadIdx.x & 31;
+    const int warp = threadIdx.x >> 5, per = tpr >> 5, first = warp & -per, lane = threadIdx.x & 31;
     if (lane == 0) slot[warp] = v;
     __syncthreads();
     return __reduce_max_sync(0xffffffffu, lane < per ? slot[first + lane] : 0u);
@@ -388,6 +447,9 @@ struct RopeArgs {
     float magnitude;
 };
 constexpr int kRopeMaxDim = 512;
+// shared-memory place of angle i: two more after every eight, so that threads which read eight each hit different banks
+__device__ __forceinline__ int rope_at(int i) { return i + 2 * (i >> 3); }
+constexpr int kRopeAngles = kRopeMaxDim / 2 + kRopeMaxDim / 8;
 
 __device__ __forceinline__ void rope_angles(const RopeArgs& p, long long token, float2* cs) {
     for (int i = threadIdx.x; i < p.rot / 2; i += blockDim.x) {
@@ -395,7 +457,7 @@ __device__ __forceinline__ void rope_angles(const RopeArgs& p, long long token, 
         a -= rint(a);
         float s, c;
         sincospif(2.0f * static_cast<float>(a), &s, &c);
-        cs[i] = make_float2(c * p.magnitude, s * p.magnitude);
+        cs[rope_at(i)] = make_float2(c * p.magnitude, s * p.magnitude);
     }
 }
 
@@ -421,7 +483,7 @@ __device__ __forceinline__ long long rope_slot(const RopeArgs& p, long long toke
 }
 
 __global__ void rope_qkv_any_kernel(const RopeArgs p) {
-    __shared__ float2 cs[kRopeMaxDim / 2];
+    __shared__ __align__(16) float2 cs[kRopeAngles];
     const long long token = blockIdx.x;
     rope_angles(p, token, cs);
     __syncthreads();
@@ -440,7 +502,7 @@ __global__ void rope_qkv_any_kernel(const RopeArgs p) {
             const bool second = p.interleaved ? (d & 1) != 0 : d >= half;
             const int apart = p.interleaved ? 1 : half;
             const float other = value(second ? e - apart : e + apart);
-            const float2 w = cs[pair];
+            const float2 w = cs[rope_at(pair)];
             o = second ? o * w.x + other * w.y : o * w.x - other * w.y;
         }
         store1(dst, p.out_type, at + d, o);
@@ -452,7 +514,7 @@ __global__ void rope_qkv_any_kernel(const RopeArgs p) {
 // first step's loads are issued before the angles are computed.
 template <int XT, int OT>
 __global__ void rope_qkv_vec_kernel(const RopeArgs p) {
-    __shared__ float2 cs[kRopeMaxDim / 2];
+    __shared__ __align__(16) float2 cs[kRopeAngles];
     const long long token = blockIdx.x;
     const int per = p.dim / 16, nrot = p.rot / 16, units = (p.heads + 2 * p.kv_heads) * per;
     auto place = [&](int u, int& head, int& d0, int& d1) {
@@ -500,7 +562,7 @@ __global__ void rope_qkv_vec_kernel(const RopeArgs p) {
             if (p.interleaved) {
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const float2 wa = cs[8 * c_now + j], wb = cs[8 * c_now + 4 + j];
+                    const float2 wa = cs[rope_at(8 * c_now) + j], wb = cs[rope_at(8 * c_now) + 4 + j];
                     const float a0 = a[2 * j], a1 = a[2 * j + 1], b0 = b[2 * j], b1 = b[2 * j + 1];
                     a[2 * j] = a0 * wa.x - a1 * wa.y;
                     a[2 * j + 1] = a1 * wa.x + a0 * wa.y;
@@ -510,7 +572,7 @@ __global__ void rope_qkv_vec_kernel(const RopeArgs p) {
             } else {
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
-                    const float2 w = cs[8 * c_now + j];
+                    const float2 w = cs[rope_at(8 * c_now) + j];
                     const float a0 = a[j];
                     a[j] = a0 * w.x - b[j] * w.y;
                     b[j] = b[j] * w.x + a0 * w.y;
