@@ -149,10 +149,11 @@ static int launch_i8gemm_pair(const void* A, long long lda, const void* B, long 
     return launch_error("i8gemm_pair_kernel launch");
 }
 
-// how many ranges of k: until the launch has a CTA for every SM, each range at least four stages long
-static int i8_split(long long tiles, int kblocks, int sm_count, int most) {
+// how many ranges of k, at most 8 (a cluster): while the launch has no more CTAs than `slots` and a range no fewer than
+// `least` stages
+static int i8_split(long long tiles, int kblocks, int slots, int least) {
     int s = 1;
-    while (s < most && tiles * s * 2 <= sm_count && kblocks / (2 * s) >= 4) s *= 2;
+    while (s < 8 && tiles * s * 2 <= slots && kblocks / (2 * s) >= least) s *= 2;
     return s;
 }
 
@@ -350,13 +351,23 @@ TK_API int tk_i8gemm(const void* A, long long lda, const float* scale_a, const v
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const int kblocks = (K + kI8BK - 1) / kI8BK;
     const long long tn = (N + 127) / 128;
-    if (M <= 16) return launch_i8gemm<16, 5, true>(A, lda, B, ldb, p, i8_split(tn, kblocks, 2 * d->sm_count, 8), st);
-    if (M <= 32) return launch_i8gemm<32, 5, true>(A, lda, B, ldb, p, i8_split(tn, kblocks, 2 * d->sm_count, 8), st);
-    if (M <= 64) return launch_i8gemm<64, 4, true>(A, lda, B, ldb, p, i8_split(tn, kblocks, 2 * d->sm_count, 8), st);
+    // Few tokens: the weights' bytes are the time.  Two CTAs per SM, ranges of at least eight stages (16 x 8192 x 4096: 12.0 us
+    // unsplit, 8.7 / 8.0 / 13.0 with 2 / 4 / 8 ranges; 1 x 4096 x 4096: 11.2, then 8.2 / 6.4 / 7.1).
+    if (M <= 64) {
+        const int split = i8_split(tn, kblocks, 2 * d->sm_count, 8);
+        if (M <= 16) return launch_i8gemm<16, 5, true>(A, lda, B, ldb, p, split, st);
+        if (M <= 32) return launch_i8gemm<32, 5, true>(A, lda, B, ldb, p, split, st);
+        return launch_i8gemm<64, 4, true>(A, lda, B, ldb, p, split, st);
+    }
     // Large products on CTA pairs: when their 256 x 256 tiles give every pair of SMs something to do
     if ((M + 255ll) / 256 * ((N + 255ll) / 256) >= d->sm_count / 2) return launch_i8gemm_pair(A, lda, B, ldb, p, d, st);
-    const long long tm = (M + 127) / 128;
-    return launch_i8gemm<128, 3, false>(A, lda, B, ldb, p, i8_split(tm * tn, kblocks, 2 * d->sm_count, 8), st);
+    // In between 128 x 128 tiles.  Joining ranges of k costs more than it gains once the tiles fill the device (300 x 4096 x
+    // 4096: 14.4 us unsplit, 15.1 with two ranges; 257 x 512 x 1024: 7.7 us, with eight 6.8).  A launch that has one CTA per
+    // SM at most takes the deeper ring.
+    const long long tiles = (M + 127ll) / 128 * tn;
+    const int split = i8_split(tiles, kblocks, d->sm_count, 1);
+    if (tiles * split <= d->sm_count) return launch_i8gemm<128, 6, false>(A, lda, B, ldb, p, split, st);
+    return launch_i8gemm<128, 3, false>(A, lda, B, ldb, p, split, st);
 }
 
 // pair i of a rotary head turns by pos * turns[i] full turns

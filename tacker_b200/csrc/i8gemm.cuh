@@ -61,6 +61,7 @@ constexpr int kI8BK = 128;  // bytes of k per stage
 // ---- output ----------------------------------------------------------------------------------------------------
 constexpr int kI8OutPitch = 36;                       // floats per staged row: conflict-free by rows and by columns
 constexpr int kI8OutBytes = 32 * kI8OutPitch * 4;     // one warp's staging
+constexpr int kI8PartPitch = 132;                     // integers per row of 128 partial sums
 
 // 32 x 32 sums of a warp (one row per lane) on their way to out rows row0 .., columns col0 ..: times the row's scale into
 // shared memory, then times the column's scale and stored with neighbouring lanes on neighbouring columns.  A row per lane
@@ -108,7 +109,7 @@ struct I8Smem {
     static constexpr int kABytes = 128 * kI8BK;
     static constexpr int kBBytes = BN * kI8BK;
     static constexpr int kStageBytes = kABytes + kBBytes;
-    static constexpr int kPartBytes = 128 * (BN + 1) * 4;  // partial sums of a range of k, over the drained stages
+    static constexpr int kPartBytes = 128 * kI8PartPitch * 4;  // partial sums of a range of k, over the drained stages
     static constexpr int kRing = STAGES * kStageBytes;
     static constexpr int kBarOffset = ((kRing > kPartBytes ? kRing : kPartBytes) + 7) / 8 * 8;
     static_assert(4 * kI8OutBytes <= kRing, "the output warps' staging fits over the drained stages");
@@ -117,9 +118,9 @@ struct I8Smem {
     static constexpr int kBytes = kAbortOffset + 4;
 };
 
-__device__ __forceinline__ int ld_shared_cluster_s32(uint32_t addr) {
-    int v;
-    asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+__device__ __forceinline__ int4 ld_shared_cluster_v4(uint32_t addr) {
+    int4 v;
+    asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
     return v;
 }
 
@@ -221,8 +222,10 @@ i8gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant_
     const uint32_t t_lane = tmem + (static_cast<uint32_t>(q * 32) << 16);
     const int r = row_a + q * 32 + lane;  // this thread's row of the MMA
     if (split > 1) {
-        // the partial sums lie in shared memory so that the lanes that finish them read and store neighbours: with SWAP an
-        // output row runs along the rows of the MMA, otherwise along its columns
+        // partial sums as rows of 128 consecutive outputs of one token: with SWAP those run along the rows of the MMA
+        static_assert(SWAP || BN == 128, "128 outputs per row");
+        constexpr int kTokens = SWAP ? BN : 128;
+        const int token0 = SWAP ? row_b : row_a, col0 = SWAP ? row_a : row_b;
         int* part = reinterpret_cast<int*>(smem);
         if (warp >= 2 && good) {
 #pragma unroll 1
@@ -230,44 +233,56 @@ i8gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant_
                 uint32_t v[32];
                 tmem_ld_32x32(t_lane + c, v);
                 tmem_ld_wait();
+                if (SWAP) {
 #pragma unroll
-                for (int j = 0; j < 32; ++j)
-                    if (c + j < BN) part[SWAP ? (c + j) * 128 + q * 32 + lane : (q * 32 + lane) * (BN + 1) + c + j] = static_cast<int>(v[j]);
+                    for (int j = 0; j < 32; ++j)
+                        if (c + j < BN) part[(c + j) * kI8PartPitch + q * 32 + lane] = static_cast<int>(v[j]);
+                } else {
+                    uint4* dst = reinterpret_cast<uint4*>(part + (q * 32 + lane) * kI8PartPitch + c);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) dst[j] = make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+                }
             }
         }
         __syncwarp();
         cluster_arrive();
         cluster_wait();
         if (warp >= 2 && good) {
-            if (SWAP) {
-                const float sr = r < p.N ? p.scale_b[r] : 0.0f, b = p.bias && r < p.N ? p.bias[r] : 0.0f;
-                const int share = BN / split;
-#pragma unroll 4
-                for (int c = rank * share; c < (rank + 1) * share; ++c) {
-                    const int token = row_b + c;
-                    if (token >= p.M) break;
-                    int sum = 0;
-                    for (int s = 0; s < split; ++s)
-                        sum += ld_shared_cluster_s32(mapa_shared(smem_base + 4u * (c * 128 + q * 32 + lane), s));
-                    if (r < p.N)
-                        store1(p.out, p.out_type, token * p.ld_out + r, static_cast<float>(sum) * p.scale_a[token] * sr + b);
-                }
-            } else {
-                const int share = 128 / split;
-                for (int i = rank * share + q; i < (rank + 1) * share; i += 4) {
-                    const int token = row_a + i;
-                    if (token >= p.M) break;
-                    const float sa = p.scale_a[token];
+            // each CTA finishes an equal share of the tokens, each lane four neighbouring outputs
+            const int col = col0 + 4 * lane, share = kTokens / split;
+            float sc[4], b[4];
 #pragma unroll
-                    for (int c = lane; c < BN; c += 32) {
-                        const int col = row_b + c;
-                        if (col >= p.N) break;
-                        int sum = 0;
-                        for (int s = 0; s < split; ++s)
-                            sum += ld_shared_cluster_s32(mapa_shared(smem_base + 4u * (i * (BN + 1) + c), s));
-                        store1(p.out, p.out_type, token * p.ld_out + col,
-                               static_cast<float>(sum) * sa * __ldg(p.scale_b + col) + (p.bias ? __ldg(p.bias + col) : 0.0f));
-                    }
+            for (int j = 0; j < 4; ++j) {
+                sc[j] = col + j < p.N ? __ldg(p.scale_b + col + j) : 0.0f;
+                b[j] = p.bias && col + j < p.N ? __ldg(p.bias + col + j) : 0.0f;
+            }
+#pragma unroll 2
+            for (int i = rank * share + q; i < (rank + 1) * share; i += 4) {
+                const int token = token0 + i;
+                if (token >= p.M) break;
+                const uint32_t at = smem_base + 4u * (i * kI8PartPitch + 4 * lane);
+                int4 x[8];
+#pragma unroll
+                for (int s = 0; s < 8; ++s)
+                    if (s < split) x[s] = ld_shared_cluster_v4(mapa_shared(at, s));
+                int4 sum = x[0];
+#pragma unroll
+                for (int s = 1; s < 8; ++s)
+                    if (s < split) sum.x += x[s].x, sum.y += x[s].y, sum.z += x[s].z, sum.w += x[s].w;
+                const float sa = __ldg(p.scale_a + token);
+                const float o[4] = {static_cast<float>(sum.x) * sa * sc[0] + b[0], static_cast<float>(sum.y) * sa * sc[1] + b[1],
+                                    static_cast<float>(sum.z) * sa * sc[2] + b[2], static_cast<float>(sum.w) * sa * sc[3] + b[3]};
+                const long long to = token * p.ld_out + col;
+                if (p.vec && col + 4 <= p.N) {
+                    if (p.out_type == kF32)
+                        *reinterpret_cast<float4*>(static_cast<float*>(p.out) + to) = make_float4(o[0], o[1], o[2], o[3]);
+                    else
+                        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + to) =
+                            make_uint2(pack2(o[0], o[1], p.out_type), pack2(o[2], o[3], p.out_type));
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        if (col + j < p.N) store1(p.out, p.out_type, to + j, o[j]);
                 }
             }
         }

@@ -405,9 +405,27 @@ __global__ void quantize_rows_kernel(const QuantArgs p, const int tpr) {
         if (c >= p.cols) continue;
         uint32_t w[2] = {0u, 0u};
         if (usable) {
+            // x / s to the nearest integer by adding 1.5 * 2^23, whose last bits then are the integer; the largest
+            // remainder of the eight says whether any lies so near a border that the exact rule has to decide
+            const float magic = 12582912.0f;
+            float far = 0.0f;
+            uint32_t bits[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-                w[j >> 2] |= (static_cast<uint32_t>(row_code(v[i][j], s, inv)) & 0xffu) << (8 * (j & 3));
+            for (int j = 0; j < 8; j += 2) {
+                float kx = v[i][j], ky = v[i][j + 1];
+                fma2(kx, ky, inv, inv, magic, magic);
+                bits[j] = __float_as_uint(kx), bits[j + 1] = __float_as_uint(ky);
+                add2(kx, ky, -magic, -magic);
+                fma2(kx, ky, -s, -s, v[i][j], v[i][j + 1]);
+                far = fmaxf(far, fmaxf(fabsf(kx), fabsf(ky)));
+            }
+            if (2.0f * far >= s) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) bits[j] = static_cast<uint32_t>(row_code(v[i][j], s, inv));
+            }
+#pragma unroll
+            for (int j = 0; j < 8; j += 4)
+                w[j >> 2] = __byte_perm(__byte_perm(bits[j], bits[j + 1], 0x0040), __byte_perm(bits[j + 2], bits[j + 3], 0x0040), 0x5410);
         }
         *reinterpret_cast<uint2*>(p.codes + row * p.ld_codes + c) = make_uint2(w[0], w[1]);
     }
