@@ -84,22 +84,70 @@ static int with_type(int type, F f) {
     return f(std::integral_constant<int, kBF16>());
 }
 
-// 8-bit matrix [rows][k], k contiguous, leading dimension ld bytes; box = 128 bytes x box_rows, 128-byte swizzle
-static int make_tmap_i8(CUtensorMap* m, const void* base, int rows, int k, long long ld, int box_rows) {
+// Tensor maps with 128-byte swizzle and zero fill.  Encoding one takes the driver about 1.5 us, as much as a launch, and a
+// serving loop asks for the same shapes again and again: each host thread keeps the last eight shapes it encoded and only
+// puts the buffer's address in.
+typedef CUresult (*ReplaceAddressFn)(CUtensorMap*, void*);
+struct TmapShape {
+    cuuint64_t dims[3], strides[2];
+    cuuint32_t box[3];
+    int type, rank;
+};
+static int make_tmap_cached(CUtensorMap* m, const void* base, const TmapShape& shape) {
+    static thread_local struct {
+        TmapShape shape[8];
+        CUtensorMap map[8];
+        int n = 0, next = 0;
+    } kept;
+    static const ReplaceAddressFn replace = [] {
+        void* fn = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        const bool ok = cudaGetDriverEntryPoint("cuTensorMapReplaceAddress", &fn, cudaEnableDefault, &q) == cudaSuccess &&
+                        q == cudaDriverEntryPointSuccess;
+        return ok ? reinterpret_cast<ReplaceAddressFn>(fn) : nullptr;
+    }();
+    for (int i = 0; replace && i < kept.n; ++i) {
+        if (std::memcmp(&kept.shape[i], &shape, sizeof(shape)) != 0) continue;
+        *m = kept.map[i];
+        if (replace(m, const_cast<void*>(base)) == CUDA_SUCCESS) return TK_OK;
+    }
     int rc = get_encoder();
     if (rc != TK_OK) return rc;
-    cuuint64_t dims[2] = {static_cast<cuuint64_t>(k), static_cast<cuuint64_t>(rows)};
-    cuuint64_t strides[1] = {static_cast<cuuint64_t>(ld)};
-    cuuint32_t box[2] = {kI8BK, static_cast<cuuint32_t>(box_rows)};
-    cuuint32_t estr[2] = {1, 1};
-    CUresult r = g_encode(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr,
-                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    const cuuint32_t estr[3] = {1, 1, 1};
+    CUresult r = g_encode(m, static_cast<CUtensorMapDataType>(shape.type), static_cast<cuuint32_t>(shape.rank),
+                          const_cast<void*>(base), shape.dims, shape.strides, shape.box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) {
-        t_last_error = "cuTensorMapEncodeTiled (8-bit matrix) failed with CUresult " + std::to_string(static_cast<int>(r));
+        t_last_error = "cuTensorMapEncodeTiled failed with CUresult " + std::to_string(static_cast<int>(r));
         return TK_ERR_CUDA;
     }
+    kept.shape[kept.next] = shape;
+    kept.map[kept.next] = *m;
+    kept.next = (kept.next + 1) % 8;
+    kept.n = std::min(8, kept.n + 1);
     return TK_OK;
+}
+
+// 8-bit matrix [rows][k], k contiguous, leading dimension ld bytes; box = 128 bytes x box_rows
+static int make_tmap_i8(CUtensorMap* m, const void* base, int rows, int k, long long ld, int box_rows) {
+    TmapShape s = {};
+    s.dims[0] = static_cast<cuuint64_t>(k), s.dims[1] = static_cast<cuuint64_t>(rows);
+    s.strides[0] = static_cast<cuuint64_t>(ld);
+    s.box[0] = kI8BK, s.box[1] = static_cast<cuuint32_t>(box_rows);
+    s.type = CU_TENSOR_MAP_DATA_TYPE_UINT8, s.rank = 2;
+    return make_tmap_cached(m, base, s);
+}
+
+// 16-bit tensor [rows][heads][dim] with rows `ld` elements apart; box = 64 elements x box_heads x box_rows; elements behind
+// dim and rows behind the last arrive as zeros
+static int make_tmap_heads(CUtensorMap* m, const void* base, int type, int rows, int heads, int dim, long long ld,
+                           int box_heads, int box_rows) {
+    TmapShape s = {};
+    s.dims[0] = static_cast<cuuint64_t>(dim), s.dims[1] = static_cast<cuuint64_t>(heads), s.dims[2] = static_cast<cuuint64_t>(rows);
+    s.strides[0] = static_cast<cuuint64_t>(dim) * 2, s.strides[1] = static_cast<cuuint64_t>(ld) * 2;
+    s.box[0] = 64, s.box[1] = static_cast<cuuint32_t>(box_heads), s.box[2] = static_cast<cuuint32_t>(box_rows);
+    s.type = type == kBF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, s.rank = 3;
+    return make_tmap_cached(m, base, s);
 }
 
 template <int BN, int STAGES, bool SWAP>
@@ -155,27 +203,6 @@ static int i8_split(long long tiles, int kblocks, int slots, int least) {
     int s = 1;
     while (s < 8 && tiles * s * 2 <= slots && kblocks / (2 * s) >= least) s *= 2;
     return s;
-}
-
-// 16-bit tensor [rows][heads][dim] with rows `ld` elements apart; box = 64 elements x box_heads x box_rows, 128-byte
-// swizzle; elements behind dim and rows behind the last arrive as zeros
-static int make_tmap_heads(CUtensorMap* m, const void* base, int type, int rows, int heads, int dim, long long ld,
-                           int box_heads, int box_rows) {
-    int rc = get_encoder();
-    if (rc != TK_OK) return rc;
-    cuuint64_t dims[3] = {static_cast<cuuint64_t>(dim), static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(rows)};
-    cuuint64_t strides[2] = {static_cast<cuuint64_t>(dim) * 2, static_cast<cuuint64_t>(ld) * 2};
-    cuuint32_t box[3] = {64, static_cast<cuuint32_t>(box_heads), static_cast<cuuint32_t>(box_rows)};
-    cuuint32_t estr[3] = {1, 1, 1};
-    CUresult r = g_encode(m, type == kBF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
-                          const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    if (r != CUDA_SUCCESS) {
-        t_last_error = "cuTensorMapEncodeTiled (heads) failed with CUresult " + std::to_string(static_cast<int>(r));
-        return TK_ERR_CUDA;
-    }
-    return TK_OK;
 }
 
 constexpr int kTokenRows = 64;  // most rows (tokens x heads of a group) of a sequence for the token form
