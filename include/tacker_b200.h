@@ -455,7 +455,7 @@ int tk_quantize_rows_i8(const void* x, int x_type, long long ld_x, void* codes, 
 
 /* out[m][n] = (sum_k A[m][k] B[n][k]) * scale_a[m] * scale_b[n] + bias[n]: 8-bit signed integers A [M][K] (tokens) and
  * B [N][K] (output channels), exact 32-bit sums, fp32 scales [M] and [N], fp32 bias [N] or null, out [M][N] of out_type.
- * Any M, N and K <= 131071 (TK_ERR_SHAPE beyond: the sums would overflow); A and B 16-byte aligned, lda and ldb multiples
+ * Any M, N <= 2^30 and K <= 131071 (TK_ERR_SHAPE beyond: the sums would overflow); A and B 16-byte aligned, lda and ldb multiples
  * of 16 (TK_ERR_ALIGN). */
 int tk_i8gemm(const void* A, long long lda, const float* scale_a, const void* B, long long ldb, const float* scale_b,
               const float* bias, void* out, long long ld_out, int out_type, int M, int N, int K, void* stream);

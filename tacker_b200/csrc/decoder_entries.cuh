@@ -362,7 +362,7 @@ TK_API int tk_i8gemm(const void* A, long long lda, const float* scale_a, const v
     if (M < 0 || N < 0 || K <= 0 || !type_ok(out_type)) return TK_ERR_ARGS;
     if (M == 0 || N == 0) return TK_OK;
     if (!A || !B || !scale_a || !scale_b || !out || lda < K || ldb < K || ld_out < N) return TK_ERR_ARGS;
-    if (K > 131071) return TK_ERR_SHAPE;  // 131071 * 2^14 is the largest sum that fits 32 bits
+    if (K > 131071 || M > (1 << 30) || N > (1 << 30)) return TK_ERR_SHAPE;  // 131071 * 2^14 is the largest sum that fits 32 bits
     if (lda % 16 || ldb % 16 || !aligned16({A, B}) || !aligned_to(scale_a, 4) || !aligned_to(scale_b, 4) ||
         !aligned_to(bias, 4) || !aligned_to(out, type_bytes(out_type)))
         return TK_ERR_ALIGN;

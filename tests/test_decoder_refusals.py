@@ -96,6 +96,8 @@ def test_8_bit(ops):
                 dict(out=P + 1)):
         refused(ALIGN, call, **bad)
     refused(SHAPE, call, K=131072, lda=131072, ldb=131072)
+    refused(SHAPE, call, M=(1 << 30) + 1)
+    refused(SHAPE, call, N=(1 << 30) + 1, ld_out=1 << 31)
     call(M=0)
     call(N=0)
 

@@ -184,6 +184,53 @@ def test_attention_bad_index_arrays_stay_inside_the_tensors(cuda):
     cuda.cuda.synchronize()
 
 
+@pytest.mark.parametrize("causal", [True, False])
+def test_attention_more_items_than_sms(cuda, causal):
+    """Several hundred work items of very different lengths: every CTA takes over blocks that have not started."""
+    lens = [2500, 3, 1700, 129, 700]
+    Attention(cuda, lens, lens, 16, 16, 64, "f16", causal).call().check()
+    Attention(cuda, lens[1:], [n + 500 for n in lens[1:]], 24, 8, 128, "bf16", causal).call().check()
+
+
+@pytest.mark.parametrize("heads,kv_heads", [(128, 1), (65, 1), (130, 1), (96, 2)])
+def test_attention_large_groups(cuda, heads, kv_heads):
+    """Groups of a whole tile, of half a tile and one more, and larger than a tile."""
+    Attention(cuda, [1, 40, 3], [700, 40, 133], heads, kv_heads, 64, "f16", True).call(workspace(cuda)).check()
+
+
+def test_attention_shared_keys(cuda):
+    """Sequences that read the same rows of the cache (a common prefix), and one that reads them behind others."""
+    for q_len in ([1, 1, 1], [130, 70, 5]):
+        a = Attention(cuda, q_len, [300, 200, 250], 8, 2, 128, "bf16", True, slab=300, poison=False)
+        a.k_start = [0, 0, 50]
+        a.index[1].copy_(cuda.tensor(a.k_start, dtype=cuda.int32))
+        a.call(workspace(cuda)).check()
+
+
+def test_attention_offsets_beyond_32_bits(cuda):
+    """A cache of more than 2^31 elements whose last rows are the ones in use; new keys written there by slots."""
+    from tacker_b200 import ops
+
+    kv_heads, dim, rows = 8, 128, 2_100_100
+    for q_len in ([1, 1], [100, 33]):
+        a = Attention(cuda, q_len, [700, 320], 16, kv_heads, dim, "bf16", True, poison=False)
+        k, v = (cuda.empty(rows, kv_heads, dim, dtype=cuda.bfloat16, device="cuda") for _ in "kv")
+        a.k_start = [rows - 1100, rows - 320]
+        for s, n in zip(a.k_start, a.k_len):
+            k[s:s + n], v[s:s + n] = normal(cuda, s, n, kv_heads, dim, type="bf16"), normal(cuda, s + 1, n, kv_heads, dim, type="bf16")
+        a.k, a.v, a.rows = k, v, rows
+        a.index[1].copy_(cuda.tensor(a.k_start, dtype=cuda.int32))
+        a.call(workspace(cuda)).check()
+    x = normal(cuda, 5, 2, (2 + 2 * kv_heads) * dim)
+    q, slots, pos = cuda.zeros(2, 2, dim, dtype=cuda.bfloat16, device="cuda"), cuda.tensor([rows - 1, rows - 7], device="cuda"), cuda.zeros(2, dtype=cuda.int32, device="cuda")
+    turns = cuda.zeros(1, dtype=cuda.float64, device="cuda")
+    ops.rope_qkv(at(x), 0, x.shape[1], 0, at(pos), at(turns), 2, 0, 1.0, 2, 2, kv_heads, dim, at(q), 2 * dim, at(k), kv_heads * dim, at(v),
+                 kv_heads * dim, 2, at(slots), rows)
+    cuda.cuda.synchronize()
+    heads = x.view(2, -1, dim).bfloat16()
+    assert cuda.equal(k[slots], heads[:, 2:2 + kv_heads]) and cuda.equal(v[slots], heads[:, 2 + kv_heads:])
+
+
 # ---- rotary heads --------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("x_type,out_type", [("f32", "f16"), ("f32", "bf16"), ("f16", "f16"), ("bf16", "bf16"), ("f16", "f32")])
 @pytest.mark.parametrize("dim,rot", [(128, 128), (128, 64), (64, 64), (80, 32), (96, 0), (64, 20), (72, 72), (6, 4), (256, 256)])
@@ -494,6 +541,25 @@ def test_block_captured_and_replayed(cuda):
         for x, y in zip(got, b.outputs()):
             assert cuda.equal(x, y)
         b.check()
+
+
+def test_two_streams_at_once(cuda):
+    """Blocks of single tokens and of prompts on two streams with buffers of their own, over and over: each gives what it
+    gives alone."""
+    blocks = [Block(cuda, [1] * 7, [3, 64, 200, 7, 0, 31, 90]), Block(cuda, [100, 3, 37, 80], [0, 20, 0, 5])]
+    alone = []
+    for b in blocks:
+        b.run()
+        cuda.cuda.synchronize()
+        alone.append(b.outputs())
+    streams = [cuda.cuda.Stream() for _ in blocks]
+    for _ in range(20):
+        for b, s in zip(blocks, streams):
+            b.run(s.cuda_stream)
+    cuda.cuda.synchronize()
+    for b, want in zip(blocks, alone):
+        for x, y in zip(b.outputs(), want):
+            assert cuda.equal(x, y)
 
 
 def test_no_wait_ran_out(cuda):
