@@ -3,11 +3,16 @@
 //
 // Rows.  The query heads that share a key head are rows of one tile: a tile has 128 / group tokens x group heads, token
 // after token, so that a key tile fetched once serves the whole group and short sequences still fill rows.  One work item
-// is two tiles (256 rows) of one sequence and key head; one persistent CTA per SM walks the items.
+// is two tiles (256 rows) of one sequence and key head; one persistent CTA per SM takes items until none is left.
 //
-//   warps 0..3, 4..7  softmax of tile 0 and of tile 1, one row per thread; at the end of an item they write its rows
-//   warp 8            issues the MMAs of both tiles:  S = Q K^T (128 x 128, fp32, TMEM),  O += P V  with P read from TMEM
-//   warp 9            TMA: Q tiles, then K and V tiles of 128 keys through a ring
+//   warps 0..3, 4..7  softmax of tile 0 and of tile 1, one row per thread
+//   warps 8..11       write the rows of finished tiles
+//   warp 12           issues the MMAs of both tiles:  S = Q K^T (128 x 128, fp32, TMEM),  O += P V  with P read from TMEM
+//   warp 13           TMA: Q tiles, then K and V tiles of 128 keys through a ring
+//   warp 14           finds the next item and hands it to the others
+//
+// The grid has a block for every item there can be; a CTA that is done takes over a block that has not started yet
+// (cluster launch control), so that items of different lengths even out without a counter in memory.
 //
 // While the softmax of one tile runs, the tensor cores work for the other one.  P overwrites the columns of its S.
 // The running maximum is raised (and O multiplied by what that costs, in TMEM) only when the new one exceeds it by more
@@ -20,7 +25,9 @@
 // nothing they hold (NaN included) can enter.
 //
 // Bound: per key tile and SM the two tiles take 2 x 2 x 512 cycles of the tensor pipe (head size 128) and 32768 powers of
-// two = 2048 cycles of the special-function units; both run at the same time.
+// two = 2048 cycles of the special-function units, both at the same time; measured are 3050 cycles, 1930 of them the softmax
+// of a tile (scores from tensor memory and their maximum 370, powers 1460) and 1000 from its weights to its next scores.
+// 8192 tokens x 16 heads x 128, causal: 220 us = 1250 TFLOP/s of visible products.
 #pragma once
 #include <cuda.h>
 

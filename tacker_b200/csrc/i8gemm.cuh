@@ -332,7 +332,8 @@ i8gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant_
 // CTA loads its own 128 rows of A and one half of the tile's rows of B, so that a stage of 128 k costs it 32 KB for 128 x 256
 // results instead of the 48 KB of a tile of its own: at 512 cycles a stage, 64 bytes a cycle from L2.  The roles and signals
 // are those of the fp16 role (gemm_role2.cuh): full barriers in the leader, empty barriers in both CTAs, two accumulators of
-// 256 columns so that a tile is written while the next one is summed.
+// 256 columns so that a tile is written while the next one is summed.  8192 x 8192 x 4096: 170 us = 3.2 POP/s at full clock, where
+// twice the measured bf16 rate would be 163 us; sustained it runs at 1.55 GHz under the power limit.
 __device__ __forceinline__ void umma_i8_pair_x4(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
                                                 uint32_t accumulate) {
     asm volatile(
