@@ -193,7 +193,7 @@ static int launch_i8gemm_pair(const void* A, long long lda, const void* B, long 
     const long long tiles = (p.M + 255ll) / 256 * ((p.N + 255ll) / 256);
     if (tiles > kMaxGridX) return TK_ERR_SHAPE;
     const long long pairs = std::min(tiles, static_cast<long long>(d->sm_count / 2));
-    kernel<<<static_cast<unsigned>(2 * pairs), 192, smem, st>>>(ta, tb, p);
+    kernel<<<static_cast<unsigned>(2 * pairs), kI8PairThreads, smem, st>>>(ta, tb, p);
     return launch_error("i8gemm_pair_kernel launch");
 }
 

@@ -63,11 +63,27 @@ constexpr int kI8OutPitch = 36;                       // floats per staged row: 
 constexpr int kI8OutBytes = 32 * kI8OutPitch * 4;     // one warp's staging
 constexpr int kI8PartPitch = 132;                     // integers per row of 128 partial sums
 
+// Scales and biases of the columns a lane stores of a chunk of 32: eight neighbours, or one where rows are not aligned or
+// the chunk is cut off by the matrix's edge.  Fetched before the sums are waited for.
+struct I8Cols {
+    float sc[8], b[8];
+};
+__device__ __forceinline__ bool i8_wide(const I8Args& p, int col0) { return p.vec && col0 + 32 <= p.N; }
+__device__ __forceinline__ void i8_columns(const I8Args& p, int col0, int lane, I8Cols& k) {
+    const bool wide = i8_wide(p, col0);
+    const int c = wide ? col0 + (lane & 3) * 8 : min(col0 + lane, p.N - 1);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        k.sc[i] = wide || i == 0 ? __ldg(p.scale_b + c + i) : 0.0f;
+        k.b[i] = p.bias && (wide || i == 0) ? __ldg(p.bias + c + i) : 0.0f;
+    }
+}
+
 // 32 x 32 sums of a warp (one row per lane) on their way to out rows row0 .., columns col0 ..: times the row's scale into
 // shared memory, then times the column's scale and stored with neighbouring lanes on neighbouring columns.  A row per lane
 // and store would touch 32 lines with every instruction.
 __device__ __forceinline__ void i8_store_chunk(const I8Args& p, float* stage, const uint32_t (&v)[32], float row_scale,
-                                               int row0, int col0, int lane) {
+                                               const I8Cols& k, int row0, int col0, int lane) {
     float4* mine = reinterpret_cast<float4*>(stage + lane * kI8OutPitch);
 #pragma unroll
     for (int i = 0; i < 8; ++i)
@@ -76,30 +92,23 @@ __device__ __forceinline__ void i8_store_chunk(const I8Args& p, float* stage, co
                               static_cast<float>(static_cast<int>(v[4 * i + 2])) * row_scale,
                               static_cast<float>(static_cast<int>(v[4 * i + 3])) * row_scale);
     __syncwarp();
-    if (p.vec && col0 + 32 <= p.N) {
+    if (i8_wide(p, col0)) {
         // eight columns per lane: four lanes per row, eight rows at a time
-        const int c = col0 + (lane & 3) * 8;
-        float sc[8], b[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int i = 0; i < 8; ++i) sc[i] = __ldg(p.scale_b + c + i);
-        if (p.bias) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) b[i] = __ldg(p.bias + c + i);
-        }
+        const long long at = (row0 + (lane >> 2)) * p.ld_out + col0 + (lane & 3) * 8;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int r = 8 * i + (lane >> 2);
             const float4* src = reinterpret_cast<const float4*>(stage + r * kI8OutPitch + (lane & 3) * 8);
             const float4 x = src[0], y = src[1];
-            const float o[8] = {x.x * sc[0] + b[0], x.y * sc[1] + b[1], x.z * sc[2] + b[2], x.w * sc[3] + b[3],
-                                y.x * sc[4] + b[4], y.y * sc[5] + b[5], y.z * sc[6] + b[6], y.w * sc[7] + b[7]};
-            if (row0 + r < p.M) store8(p.out, p.out_type, (row0 + r) * p.ld_out + c, o);
+            const float o[8] = {x.x * k.sc[0] + k.b[0], x.y * k.sc[1] + k.b[1], x.z * k.sc[2] + k.b[2], x.w * k.sc[3] + k.b[3],
+                                y.x * k.sc[4] + k.b[4], y.y * k.sc[5] + k.b[5], y.z * k.sc[6] + k.b[6], y.w * k.sc[7] + k.b[7]};
+            if (row0 + r < p.M) store8(p.out, p.out_type, at + 8 * i * p.ld_out, o);
         }
     } else if (col0 + lane < p.N) {
-        const int c = col0 + lane;
-        const float sc = __ldg(p.scale_b + c), b = p.bias ? __ldg(p.bias + c) : 0.0f;
         const int n = min(32, p.M - row0);
-        for (int r = 0; r < n; ++r) store1(p.out, p.out_type, (row0 + r) * p.ld_out + c, stage[r * kI8OutPitch + lane] * sc + b);
+#pragma unroll 8
+        for (int r = 0; r < n; ++r)
+            store1(p.out, p.out_type, (row0 + r) * p.ld_out + col0 + lane, stage[r * kI8OutPitch + lane] * k.sc[0] + k.b[0]);
     }
     __syncwarp();
 }
@@ -312,10 +321,12 @@ i8gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant_
 #pragma unroll 1
             for (int c = 0; c < BN && row_b + c < p.N; c += 32) {
                 uint32_t v[32];
+                I8Cols k;
                 __syncwarp();
                 tmem_ld_32x32(t_lane + c, v);
+                i8_columns(p, row_b + c, lane, k);
                 tmem_ld_wait();
-                i8_store_chunk(p, reinterpret_cast<float*>(smem + q * kI8OutBytes), v, sa, row_a + q * 32, row_b + c, lane);
+                i8_store_chunk(p, reinterpret_cast<float*>(smem + q * kI8OutBytes), v, sa, k, row_a + q * 32, row_b + c, lane);
             }
         }
     }
@@ -364,18 +375,21 @@ __device__ __forceinline__ void tma_load_2d_pair(uint32_t dst_smem, const void* 
 }
 
 struct I8PairSmem {
-    static constexpr int kStages = 6;
+    static constexpr int kStages = 5;
+    static constexpr int kOutWarps = 8;
     static constexpr int kTileBytes = 128 * kI8BK;
     static constexpr int kStageBytes = 2 * kTileBytes;
     static constexpr int kOutOffset = kStages * kStageBytes;
-    static constexpr int kBarOffset = kOutOffset + 4 * kI8OutBytes;
+    static constexpr int kBarOffset = kOutOffset + kOutWarps * kI8OutBytes;
     static constexpr int kNumBars = 2 * kStages + 4;
     static constexpr int kTmemSlotOffset = kBarOffset + kNumBars * 8;
     static constexpr int kAbortOffset = kTmemSlotOffset + 4;
     static constexpr int kBytes = kAbortOffset + 4;
 };
 
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1)
+constexpr int kI8PairThreads = 64 + 32 * I8PairSmem::kOutWarps;
+
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kI8PairThreads, 1)
 i8gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b, const I8Args p) {
     using L = I8PairSmem;
     constexpr int ST = L::kStages;
@@ -405,7 +419,7 @@ i8gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_cons
         }
         for (int a = 0; a < 2; ++a) {
             mbar_init(tfull_bar(a), 1);
-            mbar_init(tempty_bar(a), 8);  // used in the leader only: four output warps of each CTA
+            mbar_init(tempty_bar(a), 2 * L::kOutWarps);  // used in the leader only: the output warps of both CTAs
         }
         fence_mbar_init();
         tma_prefetch_desc(&tmap_a);
@@ -506,9 +520,11 @@ i8gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_cons
         }
     } else {
         // ---------------- output (both CTAs) ----------------
-        const int q = warp & 3;
+        // two warps for each 32 rows, half of the columns each: four warps took 12,000 cycles for a tile, more than the MMAs
+        // of K = 2048 take
+        const int q = warp & 3, first = (warp - 2) / 4 * 128;
         const uint32_t tempty_leader0 = mapa_shared(tempty_bar(0), 0u);
-        float* stage = reinterpret_cast<float*>(smem + L::kOutOffset + q * kI8OutBytes);
+        float* stage = reinterpret_cast<float*>(smem + L::kOutOffset + (warp - 2) * kI8OutBytes);
         uint32_t it = 0;
         bool ok = true;
         for (int tile = pair; ok && tile < tiles; tile += npairs, ++it) {
@@ -520,11 +536,17 @@ i8gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_cons
             const float sa = row0 + lane < p.M ? __ldg(p.scale_a + row0 + lane) : 0.0f;
             const uint32_t t_lane = tmem + (static_cast<uint32_t>(q * 32) << 16) + as * 256;
 #pragma unroll 1
-            for (int c = 0; c < 256 && col0 + c < p.N && row0 < p.M; c += 32) {
-                uint32_t v[32];
+            for (int c = first; c < first + 128 && col0 + c < p.N && row0 < p.M; c += 64) {
+                // two chunks on their way at once
+                uint32_t v[32], w[32];
+                I8Cols k, m;
                 tmem_ld_32x32(t_lane + c, v);
+                tmem_ld_32x32(t_lane + c + 32, w);
+                i8_columns(p, col0 + c, lane, k);
+                i8_columns(p, min(col0 + c + 32, p.N - 1), lane, m);
                 tmem_ld_wait();
-                i8_store_chunk(p, stage, v, sa, row0, col0 + c, lane);
+                i8_store_chunk(p, stage, v, sa, k, row0, col0 + c, lane);
+                if (col0 + c + 32 < p.N) i8_store_chunk(p, stage, w, sa, m, row0, col0 + c + 32, lane);
             }
             tc_fence_before_sync();
             __syncwarp();
