@@ -386,8 +386,9 @@ TK_API int tk_i8gemm(const void* A, long long lda, const float* scale_a, const v
         if (M <= 32) return launch_i8gemm<32, 5, true>(A, lda, B, ldb, p, split, st);
         return launch_i8gemm<64, 4, true>(A, lda, B, ldb, p, split, st);
     }
-    // Large products on CTA pairs: when their 256 x 256 tiles give every pair of SMs something to do
-    if ((M + 255ll) / 256 * ((N + 255ll) / 256) >= d->sm_count / 2) return launch_i8gemm_pair(A, lda, B, ldb, p, d, st);
+    // Large products on CTA pairs: when their 256 x 256 tiles give half of the pairs of SMs something to do (64 tiles: 512 x 8192
+    // x 4096 16.4 us, 19.0 in smaller tiles; 32 tiles: 300 x 4096 x 4096 15.4 us against 14.6)
+    if ((M + 255ll) / 256 * ((N + 255ll) / 256) >= d->sm_count / 4) return launch_i8gemm_pair(A, lda, B, ldb, p, d, st);
     // In between 128 x 128 tiles.  Joining ranges of k costs more than it gains once the tiles fill the device (300 x 4096 x
     // 4096: 14.4 us unsplit, 15.1 with two ranges; 257 x 512 x 1024: 7.7 us, with eight 6.8).  A launch that has one CTA per
     // SM at most takes the deeper ring.
@@ -480,7 +481,8 @@ TK_API int tk_attention_packed(const void* q, long long ld_q, const void* k, lon
         return TK_ERR_ARGS;
     if (heads % kv_heads) return TK_ERR_ARGS;
     if (n_seqs == 0 || total_q == 0) return TK_OK;
-    if (dim > 256 || static_cast<long long>(total_q) * heads > kMaxGridX) return TK_ERR_SHAPE;
+    if (dim > 256 || static_cast<long long>(total_q) * heads > kMaxGridX || total_q > (1 << 30) || kv_rows > (1 << 30))
+        return TK_ERR_SHAPE;
     if (!q || !out || !q_start || !k_start || !k_len || (kv_rows > 0 && (!k || !v))) return TK_ERR_ARGS;
     if (ld_q < static_cast<long long>(heads) * dim || ld_out < static_cast<long long>(heads) * dim ||
         ld_k < static_cast<long long>(kv_heads) * dim || ld_v < static_cast<long long>(kv_heads) * dim)

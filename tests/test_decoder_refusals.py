@@ -44,6 +44,9 @@ def test_attention(ops):
                 dict(k_len=P + 2), dict(workspace=P + 8)):
         refused(ALIGN, call, **bad)
     refused(SHAPE, call, dim=264, ld_q=8 * 264, ld_k=528, ld_v=528, ld_out=8 * 264)
+    refused(SHAPE, call, total_q=(1 << 30) + 1)
+    refused(SHAPE, call, total_q=1 << 29)  # times 8 heads
+    refused(SHAPE, call, kv_rows=(1 << 30) + 1)
     call(n_seqs=0)
     call(total_q=0)
 

@@ -396,7 +396,8 @@ def test_quantize_rows_that_have_no_scale(cuda):
 @pytest.mark.parametrize("out_type", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("M,N,K", [(1, 1, 16), (1, 128, 128), (3, 333, 48), (16, 4096, 4096), (17, 130, 2048), (33, 1000, 1040),
                                    (64, 512, 16384), (65, 64, 128), (127, 129, 130), (128, 256, 512), (130, 1234, 1040),
-                                   (300, 77, 4096), (1001, 515, 640), (512, 768, 100), (2048, 2048, 256)])
+                                   (300, 77, 4096), (1001, 515, 640), (512, 768, 100), (2048, 2048, 256),
+                                   (1537, 2305, 200), (2304, 1280, 1040), (70, 12000, 64), (1030, 8200, 16)])
 def test_i8gemm(cuda, out_type, M, N, K):
     from tacker_b200 import ops
 
