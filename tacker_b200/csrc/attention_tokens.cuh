@@ -131,9 +131,8 @@ attention_tokens_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
                 tma_load_tile(dst + L::kHalfBytes + x * L::kBoxBytes, &tmap_v, full(st), 64 * x, kv, row);
             }
         };
-        int head_stage = stage;
         if (lane == 0)
-            for (int i = 0; i < ST - 1 && i < tiles; ++i) load(i, (head_stage + i) % ST);
+            for (int i = 0; i < ST - 1 && i < tiles; ++i) load(i, (stage + i) % ST);
         // Q as A fragments
         uint32_t q[D / 16][4];
 #pragma unroll
@@ -241,8 +240,8 @@ attention_tokens_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
                 phase ^= 1u;
             }
         }
-        // the warps' results meet over the rings, which are drained
-        __syncthreads();
+        // the warps' results meet over the rings, which are drained; after a wait that ran out nothing is to be joined
+        if (!__syncthreads_and(ok)) break;
         float* acc = reinterpret_cast<float*>(smem);                            // [warp][16][D]
         float2* ml = reinterpret_cast<float2*>(acc + kTokWarps * kTokRows * D);  // [warp][16]
 #pragma unroll
