@@ -98,11 +98,12 @@ __global__ void attention_rows_kernel(const AttnArgs p) {
             if (lane + 32 * e < p.dim) o[e] = fmaf(o[e], keep, w * load1(p.v, p.type, vr + lane + 32 * e));
         m = m_new;
     }
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    const float inv = 1.0f / l;
 #pragma unroll
     for (int e = 0; e < E; ++e)
         if (lane + 32 * e < p.dim)
-            store1(p.out, p.type, row * p.ld_out + static_cast<long long>(head) * p.dim + lane + 32 * e, o[e] * inv);
+            store1(p.out, p.type, row * p.ld_out + static_cast<long long>(head) * p.dim + lane + 32 * e,
+                   l == 0.0f ? 0.0f : o[e] * inv);  // keys that score -infinity weigh zero, even where v is not finite
     if (p.lse && lane == 0)
         p.lse[static_cast<long long>(row) * p.heads + head] = l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2;
 }

@@ -65,6 +65,15 @@ __device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4],
                      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+// Four weighted values over the sum of their weights.  Without a weight the result is zero whatever v holds: keys that the
+// mask hides weigh zero, and zero times an infinity or a NaN among their values has made v NaN.
+template <int TYPE>
+__device__ __forceinline__ uint2 attn_result(const float4& v, float sum) {
+    if (sum == 0.0f) return make_uint2(0u, 0u);
+    const float inv = 1.0f / sum;
+    return make_uint2(pack2(v.x * inv, v.y * inv, TYPE), pack2(v.z * inv, v.w * inv, TYPE));
+}
+
 template <int D, int TYPE>
 __global__ void __launch_bounds__(kTokWarps * 32, 2)
 attention_tokens_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v,
@@ -281,9 +290,8 @@ attention_tokens_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
                 *reinterpret_cast<float4*>(a.part_o + slot * p.dim + d) = v;
                 if (d == 0) a.part_ml[slot] = make_float2(mm, sum);
             } else {
-                const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
                 *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + row * p.ld_out + static_cast<long long>(hd) * p.dim + d) =
-                    make_uint2(pack2(v.x * inv, v.y * inv, TYPE), pack2(v.z * inv, v.w * inv, TYPE));
+                    attn_result<TYPE>(v, sum);
                 if (d == 0 && p.lse) p.lse[row * p.heads + hd] = sum == 0.0f ? -INFINITY : (mm + log2f(sum)) * kLn2;
             }
         }
@@ -335,10 +343,9 @@ __global__ void attention_join_kernel(const AttnArgs p, const TokArgs a) {
         sum += part[w].x;
     }
     const int head = static_cast<int>(item - row * p.heads);
-    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
     if (d < p.dim)
         *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + row * p.ld_out + static_cast<long long>(head) * p.dim + d) =
-            make_uint2(pack2(v.x * inv, v.y * inv, TYPE), pack2(v.z * inv, v.w * inv, TYPE));
+            attn_result<TYPE>(v, sum);
     if (lane == 0 && p.lse) p.lse[item] = sum == 0.0f ? -INFINITY : (m + log2f(sum)) * kLn2;
 }
 

@@ -1,0 +1,48 @@
+"""Decoder-block operators at the edges of their contracts: non-finite operands, rows that see nothing, calls that tests of
+ordinary shapes do not make (B200 only)."""
+import math
+
+import pytest
+
+import decoder_ref as ref
+from test_gpu_decoder import Attention, workspace
+
+pytestmark = pytest.mark.gpu
+
+
+# ---- attention: non-finite keys and values -------------------------------------------------------------------------
+FORMS = {"prompt": dict(q=130, dim=64), "tokens": dict(q=5, dim=64), "rows": dict(q=5, dim=64, pad=1), "rows, long": dict(q=130, dim=64, pad=1)}
+
+
+@pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("form", FORMS)
+def test_attention_rows_without_a_key_are_zero_whatever_the_values_hold(cuda, form, value):
+    """Three keys behind more queries than that: the first queries see none, and give zeros and lse -infinity although the
+    keys they do not see have values that are not finite."""
+    f = dict(FORMS[form])
+    q = f.pop("q")
+    a = Attention(cuda, [q], [3], 8, 2, type="f16", causal=True, slab=16, **f)
+    a.v[0] = value
+    for w in (workspace(cuda), None):
+        a.out.fill_(7)
+        a.call(w)
+        cuda.cuda.synchronize()
+        got = a.out[:, :8 * a.dim]
+        assert bool((got[:q - 3] == 0).all()) and bool((a.lse[:q - 3] == -math.inf).all())
+        assert not bool(got[q - 3:].isfinite().any())
+        want_lse, tol_lse = ref.attention(a.q, a.k, a.v, a.q_start, a.k_start, a.k_len, a.scale, True, "f16")[1::2]
+        assert bool(((a.lse - want_lse).abs()[q - 3:] <= tol_lse[q - 3:]).all())
+
+
+@pytest.mark.parametrize("form", FORMS)
+def test_attention_keys_that_score_minus_infinity(cuda, form):
+    """Every key of the sequence scores -infinity: no weight is left, zeros and lse -infinity, also with infinite values."""
+    f = dict(FORMS[form])
+    q = f.pop("q")
+    a = Attention(cuda, [q], [200], 8, 2, type="bf16", causal=False, **f)
+    a.q.abs_().add_(0.5)
+    a.k.fill_(-math.inf)
+    a.v[7] = math.inf
+    a.call(workspace(cuda))
+    cuda.cuda.synchronize()
+    assert bool((a.out[:, :8 * a.dim] == 0).all()) and bool((a.lse == -math.inf).all())
