@@ -509,11 +509,16 @@ int tk_attention_packed(const void* q, long long ld_q, const void* k, long long 
  * tk_plan_tzgemm: cover[t] += 1 for every 64x64 tile t of the M x N result that a launch of `ctas` CTAs with
  *   super-tile width bn writes for [start, end); work[c] (optional) += super-tiles of CTA c.
  * tk_plan_stencil: planes[b*nz + k] += 1 for every plane k of bundle b some warp computes, loads[b*nz + k]
- *   (optional) += 1 for every plane streamed; split = {slabs per bundle, planes per slab} chosen for the launch. */
+ *   (optional) += 1 for every plane streamed; split = {slabs per bundle, planes per slab} chosen for the launch.
+ * tk_plan_attention: cover[kv * sum(q_len) + token] += 1 for every token and key head that a launch of `blocks` blocks of
+ *   the attention kernel for prompts works on (tile_tokens = 128 / group); CTA c of `ctas` starts as block order[c] and takes
+ *   over blocks order[c + ctas], order[c + 2 ctas] ... */
 int tk_plan_tzgemm(int M, int N, int bn, int start, int end, int ctas, int* cover, int* work);
 int tk_plan_tzgemm_m256(int M, int N, int start, int end, int ctas, int* cover); /* 256 x 256 super-tile kernel */
 int tk_plan_stencil(int nz, int blocks_start, int blocks_end, int gx, int gy, int ctas, int warps_per_cta,
                     int* planes, int* loads, int split[2]);
+int tk_plan_attention(const int* q_len, int n_seqs, int kv_heads, int tile_tokens, const int* order, int blocks, int ctas,
+                      int* cover);
 
 /* ---- MRI-Q for callers that cannot allocate device memory ----------------------------------------------
  * (No counterpart in the reference: it always cudaMallocs its buffers up front.)

@@ -214,18 +214,71 @@ struct AttnItem {
     int n[2];  // key tiles that some row of the tile sees
 };
 
-// Finds work items by index, in ascending order of calls.  Items of a sequence run from its last tokens (which see the
-// most keys) to its first, key heads innermost.  All lanes of a warp call it together.
-struct AttnWalk {
-    int base;          // first sequence of the window of 32 that the search stands at; this lane's sequence is base + lane
+// The search for a work item by its number.  Sequences are looked through in windows of 32, forward from where the last
+// search ended and from the start again for a number that lies before; the end is remembered.  `Window` holds the sequences
+// of one window: load(base) reads them, items() counts their items.
+struct AttnSeek {
+    int base = 0;             // first sequence of the window
+    long long before = 0;     // items of the sequences before it
+    long long total = 0x7fffffffffffffffll;  // all items, once a search has come to the end
+
+    // (host and device windows both: the compiler's check of where a template argument's functions may run is off)
+#pragma nv_exec_check_disable
+    template <class Window>
+    __host__ __device__ __forceinline__ bool find(long long index, int n_seqs, Window& w) {
+        if (index >= total) return false;
+        if (index < before) {
+            base = 0, before = 0;
+            w.load(base);
+        }
+        for (long long n; index >= before + (n = w.items());) {
+            before += n;
+            base += 32;
+            if (base >= n_seqs) {
+                total = before;
+                return false;
+            }
+            w.load(base);
+        }
+        return true;
+    }
+};
+
+// The course of one CTA: its own block's number, then those of the blocks it takes over, until all have started.  Blocks
+// are given out in no order that could be relied on, so each number is looked up, also after one that lies behind the last
+// item.  hand(index) does with an item what is to be done, take(index) asks for the next number (-1: none left); both are
+// false after a wait that ran out.
+#pragma nv_exec_check_disable
+template <class Find, class Hand, class Take>
+__host__ __device__ __forceinline__ bool attn_items(int index, Find find, Hand hand, Take take) {
+    while (index >= 0) {
+        if (find(index) && !hand()) return false;
+        if (!take(index)) return false;
+    }
+    return true;
+}
+
+// Place of item `at` of a sequence that has `of`: items run from its last tokens (which see the most keys) to its first, key
+// heads innermost.
+__host__ __device__ __forceinline__ void attn_item_place(int at, long long of, int kv_heads, int tile_tokens, int& kv, int& t0) {
+    kv = at % kv_heads;
+    t0 = (static_cast<int>(of) - 1 - at) / kv_heads * 2 * tile_tokens;
+}
+__host__ __device__ __forceinline__ long long attn_items_of(int q_len, int kv_heads, int tile_tokens) {
+    return static_cast<long long>((q_len + 2 * tile_tokens - 1) / (2 * tile_tokens)) * kv_heads;
+}
+
+// A window of the search in the registers of a warp, a sequence per lane; all lanes call together.
+struct AttnWindow {
+    const AttnArgs& p;
+    const int tile_tokens, lane;
     AttnSeq s;
-    long long before;  // items of the sequences before the window
     long long mine, upto;  // items of this lane's sequence, and of the window up to and with it
 
-    __device__ __forceinline__ void window(const AttnArgs& p, int tile_tokens, int lane) {
+    __device__ __forceinline__ void load(int base) {
         s.q_len = 0, s.q0 = 0, s.k0 = 0, s.k_len = 0;
         if (base + lane < p.n_seqs) s.load(p, base + lane);
-        mine = static_cast<long long>((s.q_len + 2 * tile_tokens - 1) / (2 * tile_tokens)) * p.kv_heads;
+        mine = attn_items_of(s.q_len, p.kv_heads, tile_tokens);
         upto = mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -233,27 +286,17 @@ struct AttnWalk {
             if (lane >= o) upto += u;
         }
     }
-    __device__ __forceinline__ void init(const AttnArgs& p, int tile_tokens, int lane) {
-        base = 0, before = 0;
-        window(p, tile_tokens, lane);
-    }
-    __device__ __forceinline__ bool find(const AttnArgs& p, long long index, int tile_tokens, int lane, AttnItem& it) {
-        uint32_t hit;
-        while ((hit = __ballot_sync(0xffffffffu, before + upto > index)) == 0u) {
-            before += __shfl_sync(0xffffffffu, upto, 31);
-            base += 32;
-            if (base >= p.n_seqs) return false;
-            window(p, tile_tokens, lane);
-        }
-        const int l = __ffs(hit) - 1;
+    __device__ __forceinline__ long long items() const { return __shfl_sync(0xffffffffu, upto, 31); }
+    // item number `index` of the window
+    __device__ __forceinline__ void item(long long index, AttnItem& it) const {
+        const int l = __ffs(__ballot_sync(0xffffffffu, upto > index)) - 1;
         it.s.q0 = __shfl_sync(0xffffffffu, s.q0, l);
         it.s.q_len = __shfl_sync(0xffffffffu, s.q_len, l);
         it.s.k0 = __shfl_sync(0xffffffffu, s.k0, l);
         it.s.k_len = __shfl_sync(0xffffffffu, s.k_len, l);
         const long long of = __shfl_sync(0xffffffffu, mine, l);
-        const int at = static_cast<int>(index - before - (__shfl_sync(0xffffffffu, upto, l) - of));
-        it.kv = at % p.kv_heads;
-        it.t0 = (static_cast<int>(of) - 1 - at) / p.kv_heads * 2 * tile_tokens;
+        attn_item_place(static_cast<int>(index - (__shfl_sync(0xffffffffu, upto, l) - of)), of, p.kv_heads, tile_tokens, it.kv,
+                        it.t0);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const int first = it.t0 + h * tile_tokens;
@@ -262,7 +305,6 @@ struct AttnWalk {
             if (p.causal) keys = min(keys, max(0, last + 1 + it.s.k_len - it.s.q_len));
             it.n[h] = last < first ? 0 : (keys + kAttnKeys - 1) / kAttnKeys;
         }
-        return true;
     }
 };
 
@@ -382,12 +424,33 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
       fewer_registers<kAttnOtherRegs>();
       if (warp == 14) {
         // ---------------- items ----------------
-        AttnWalk walk;
-        walk.init(p, tile_tokens, lane);
-        int index = blockIdx.x;
+        AttnWindow window = {p, tile_tokens, lane};
+        window.load(0);
+        AttnSeek seek;
         uint32_t claim_phase = 0;
-        bool ok = true, open = true;  // open: there may be blocks that have not started
-        auto claim = [&]() {
+        auto publish = [&](int t0) {
+            if (lane == 0) {
+                int4* dst = reinterpret_cast<int4*>(smem + L::kItemOffset);
+                dst[0] = make_int4(it.s.q0, it.s.q_len, it.s.k0, it.s.k_len);
+                dst[1] = make_int4(it.kv, t0, it.n[0], it.n[1]);
+                mbar_arrive(item_full);
+            }
+            __syncwarp();
+        };
+        auto find = [&](int index) {
+            if (!seek.find(index, p.n_seqs, window)) return false;
+            window.item(index - seek.before, it);
+            return true;
+        };
+        // the next one is claimed when the loads of this one are on their way and everyone has read it: earlier, and a CTA
+        // that is at a long item would hold another that nobody else can take
+        auto hand = [&]() {
+            publish(it.t0);
+            const bool read = wait(item_empty, item_phase, DEV_TIMEOUT_EMPTY);
+            item_phase ^= 1u;
+            return read;
+        };
+        auto take = [&](int& index) {
             if (lane == 0) {
                 fence_proxy_async_smem();  // the last result has been read
                 mbar_arrive_expect_tx(claim_bar, 16);
@@ -396,31 +459,12 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
             __syncwarp();
             if (!wait(claim_bar, claim_phase, DEV_TIMEOUT_FULL)) return false;
             claim_phase ^= 1u;
-            const int taken = claim_result(base + L::kClaimOffset);
+            index = claim_result(base + L::kClaimOffset);
             __syncwarp();
-            open = taken >= 0;
-            if (open && taken < index) walk.init(p, tile_tokens, lane);  // the walk only goes forward
-            index = taken;
             return true;
         };
-        while (ok) {
-            const bool found = walk.find(p, index, tile_tokens, lane, it);
-            if (lane == 0) {
-                int4* dst = reinterpret_cast<int4*>(smem + L::kItemOffset);
-                dst[0] = make_int4(it.s.q0, it.s.q_len, it.s.k0, it.s.k_len);
-                dst[1] = make_int4(it.kv, found ? it.t0 : -1, it.n[0], it.n[1]);
-                mbar_arrive(item_full);
-            }
-            if (!found) break;
-            // the next one is claimed when the loads of this one are on their way and everyone has read it: earlier, and
-            // a CTA that is at a long item would hold another that nobody else can take
-            ok = wait(item_empty, item_phase, DEV_TIMEOUT_EMPTY);
-            item_phase ^= 1u;
-            if (!ok) break;
-            ok = claim();
-            if (!open) index = 0x7fffffff;  // no block has this number: the walk ends
-        }
-        while (ok && open) ok = claim();  // blocks behind the last item need not start
+        it.s.q0 = it.s.q_len = it.s.k0 = it.s.k_len = it.kv = it.n[0] = it.n[1] = 0;
+        if (attn_items(blockIdx.x, find, hand, take)) publish(-1);  // the end
       } else if (warp == 13) {
         // ---------------- TMA producer ----------------
         int stage = 0;

@@ -1694,6 +1694,61 @@ TK_API int tk_plan_stencil(int nz, int blocks_start, int blocks_end, int gx, int
     return TK_OK;
 }
 
+// cover[kv * total + token] += 1 for every token (counted over the sequences in turn) and key head of the items that `ctas`
+// CTAs of the attention kernel for prompts work on, where the launch has `blocks` blocks: CTA c starts as block order[c] and
+// takes over the blocks order[c + ctas], order[c + 2 ctas] ...
+TK_API int tk_plan_attention(const int* q_len, int n_seqs, int kv_heads, int tile_tokens, const int* order, int blocks,
+                             int ctas, int* cover) {
+    if (!q_len || !order || !cover || n_seqs < 1 || kv_heads < 1 || tile_tokens < 1 || blocks < 1 || ctas < 1)
+        return TK_ERR_ARGS;
+    long long total = 0;
+    for (int i = 0; i < n_seqs; ++i) {
+        if (q_len[i] < 0) return TK_ERR_ARGS;
+        total += q_len[i];
+    }
+    struct Window {
+        const int* q_len;
+        int n_seqs, kv_heads, tile_tokens, base;
+        long long of(int i) const { return i < n_seqs ? attn_items_of(q_len[i], kv_heads, tile_tokens) : 0; }
+        void load(int first) { base = first; }
+        long long items() const {
+            long long n = 0;
+            for (int i = base; i < base + 32; ++i) n += of(i);
+            return n;
+        }
+    };
+    for (int c = 0; c < ctas && c < blocks; ++c) {
+        Window w = {q_len, n_seqs, kv_heads, tile_tokens, 0};
+        AttnSeek seek;
+        long long at = c;
+        int now = 0;
+        attn_items(
+            order[c],
+            [&](int index) {
+                now = index;
+                return seek.find(index, n_seqs, w);
+            },
+            [&]() {
+                long long rest = now - seek.before, first = 0;
+                int i = 0;
+                for (; i < w.base || rest >= w.of(i); ++i) {
+                    if (i >= w.base) rest -= w.of(i);
+                    first += q_len[i];
+                }
+                int kv, t0;
+                attn_item_place(static_cast<int>(rest), w.of(i), kv_heads, tile_tokens, kv, t0);
+                for (int t = t0; t < t0 + 2 * tile_tokens && t < q_len[i]; ++t) cover[kv * total + first + t] += 1;
+                return true;
+            },
+            [&](int& index) {
+                at += ctas;
+                index = at < blocks ? order[at] : -1;
+                return true;
+            });
+    }
+    return TK_OK;
+}
+
 // Diagnostic builds (-DTK_TRACE) only: the per-CTA phase timestamps of the last tzgemm launch on CTA pairs
 // (512 CTAs x 16 values, layout in gemm_role2.cuh).
 #ifdef TK_TRACE
