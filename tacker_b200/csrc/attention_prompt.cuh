@@ -733,6 +733,7 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
                 limit = min(limit, max(0, first + token + 1 + it.s.k_len - it.s.q_len));
                 tile_limit = min(tile_limit, max(0, first + 1 + it.s.k_len - it.s.q_len));
             }
+            const bool stored = token < tile_tokens && first + token < it.s.q_len;
             const int n = h ? it.n[1] : it.n[0];
             float m = -INFINITY, l = 0.0f;
             for (int j = 0; j < n; ++j) {
@@ -764,8 +765,10 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
                     m = top;
                 } else {
                     // a row's own scores decide, so that its result does not depend on its neighbours'; true from -infinity
-                    // and for NaN as well
-                    const bool raise = !((top - m) * p.scale_log2 <= 8.0f);
+                    // and for NaN as well.  Rows that are not stored have no say: what lies there (of other sequences, behind
+                    // them, or in shared memory where no box reaches) may hold NaN, and would have its warp rescale for
+                    // every key tile (16384 keys, 65 tokens and NaN behind them: 233 us instead of 206)
+                    const bool raise = stored && !((top - m) * p.scale_log2 <= 8.0f);
                     if (__any_sync(0xffffffffu, raise)) {
                         // the scores of this tile follow the product that last added to O: O is at rest
                         const float up = raise ? max2(m, top) : m;
