@@ -187,17 +187,26 @@ i8gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant_
         if (lane == 0) {
             int stage = 0;
             uint32_t phase = 0;
-            for (int kb = kb0; kb < kb1; ++kb) {
-                if (!mbar_wait(empty_bar(stage), phase ^ 1u, abort_flag, p.status, DEV_TIMEOUT_EMPTY)) break;
-                mbar_arrive_expect_tx(full_bar(stage), L::kStageBytes);
-                const uint32_t dst = smem_base + stage * L::kStageBytes;
-                tma_load_2d(dst, &tmap_a, full_bar(stage), kb * kI8BK, row_a);
-                tma_load_2d(dst + L::kABytes, &tmap_b, full_bar(stage), kb * kI8BK, row_b);
+            bool ok = true;
+            auto advance = [&]() {
                 if (++stage == STAGES) {
                     stage = 0;
                     phase ^= 1u;
                 }
+            };
+            for (int kb = kb0; kb < kb1; ++kb) {
+                ok = mbar_wait(empty_bar(stage), phase ^ 1u, abort_flag, p.status, DEV_TIMEOUT_EMPTY);
+                if (!ok) break;
+                mbar_arrive_expect_tx(full_bar(stage), L::kStageBytes);
+                const uint32_t dst = smem_base + stage * L::kStageBytes;
+                tma_load_2d(dst, &tmap_a, full_bar(stage), kb * kI8BK, row_a);
+                tma_load_2d(dst + L::kABytes, &tmap_b, full_bar(stage), kb * kI8BK, row_b);
+                advance();
             }
+            // the last commits arrive on the empty barriers asynchronously, and nothing orders them before the one on done_bar:
+            // the CTA must not retire before they have landed
+            for (int s = 0; s < STAGES && ok; ++s, advance())
+                ok = mbar_wait(empty_bar(stage), phase ^ 1u, abort_flag, p.status, DEV_TIMEOUT_EMPTY);
         }
     } else if (warp == 1) {
         if (lane == 0) {
@@ -222,7 +231,7 @@ i8gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant_
             if (ok) umma_commit(done_bar);
         }
     }
-    // the accumulator is complete: so have all loads landed and all commits before this one been signalled
+    // the accumulator is complete, so all loads have landed
     __syncwarp();
     const bool good = mbar_wait(done_bar, 0, abort_flag, p.status, DEV_TIMEOUT_TMEM_FULL);
     tc_fence_after_sync();

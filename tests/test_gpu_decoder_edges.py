@@ -70,3 +70,25 @@ def test_attention_rows_that_are_not_stored_cost_nothing(cuda, q, heads, kv_head
     assert cuda.equal(out["zero"], out["nan"])
     a.check()
     assert best["nan"] <= 1.05 * best["zero"], best
+
+
+# ---- 8-bit products ------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("M,N,K", [(1, 4096, 16), (16, 512, 1024), (64, 300, 400), (130, 1234, 1040), (65, 64, 128)])
+def test_i8gemm_launches_one_behind_the_other(cuda, M, N, K):
+    """CTAs that follow each other on an SM: hundreds of launches with nothing between them give what the first one gives,
+    with fewer blocks of k than stages and with more."""
+    from tacker_b200 import ops
+
+    g = cuda.Generator(device="cuda")
+    g.manual_seed(M)
+    a, b = (cuda.randint(-128, 128, (r, K), generator=g, device="cuda", dtype=cuda.int8) for r in (M, N))
+    sa, sb = cuda.rand(M, generator=g, device="cuda"), cuda.rand(N, generator=g, device="cuda")
+    outs = [cuda.full((M, N), 7.0, device="cuda") for _ in range(300)]
+    cuda.cuda.synchronize()
+    for o in outs:
+        ops.i8gemm(a.data_ptr(), K, sa.data_ptr(), b.data_ptr(), K, sb.data_ptr(), 0, o.data_ptr(), N, 0, M, N, K)
+    cuda.cuda.synchronize()
+    want, tol = ref.i8gemm(a, sa, b, sb, None, "f32")
+    assert bool(((outs[0].double() - want).abs() <= tol).all())
+    assert all(cuda.equal(o, outs[0]) for o in outs)
+    assert ops.device_status() == 0
