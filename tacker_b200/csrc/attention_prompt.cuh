@@ -203,7 +203,8 @@ struct AttnSmem {
     static constexpr int kNumBars = 2 * kStages + 16 + 3;
     static constexpr int kTmemSlotOffset = kBarOffset + kNumBars * 8;
     static constexpr int kAbortOffset = kTmemSlotOffset + 4;
-    static constexpr int kBytes = kAbortOffset + 4;
+    static constexpr int kProgressOffset = kAbortOffset + 4;
+    static constexpr int kBytes = kProgressOffset + 4;
 };
 
 // One work item: two tiles of query rows of one sequence and key head.
@@ -361,10 +362,12 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
     const uint32_t item_full = bars + 8u * (2 * ST + 16), item_empty = item_full + 8, claim_bar = item_full + 16;
     volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + L::kTmemSlotOffset);
     volatile uint32_t* abort_flag = reinterpret_cast<volatile uint32_t*>(smem + L::kAbortOffset);
+    volatile uint32_t* progress = reinterpret_cast<volatile uint32_t*>(smem + L::kProgressOffset);  // tiles asked for
 
     if (warp == 12) {
         if (lane == 0) {
             *abort_flag = 0u;
+            *progress = 0u;
             for (int s = 0; s < ST; ++s) {
                 mbar_init(kv_full(s), 1);
                 mbar_init(kv_empty(s), 1);
@@ -403,11 +406,15 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
     auto wait = [&](uint32_t bar, uint32_t parity, unsigned code) {
         return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, status, code)) != 0;
     };
+    // a wait that spans an item, whose length has no bound: the producer's steps keep it alive
+    auto wait_item = [&](uint32_t bar, uint32_t parity, unsigned code) {
+        return __all_sync(0xffffffffu, mbar_wait_progress(bar, parity, abort_flag, status, code, progress)) != 0;
+    };
     // the next item, for the warps that work on items; false at the end
     uint32_t item_phase = 0;
     AttnItem it;
     auto next_item = [&](bool release) {
-        if (!wait(item_full, item_phase, DEV_TIMEOUT_FULL)) return false;
+        if (!wait_item(item_full, item_phase, DEV_TIMEOUT_FULL)) return false;
         const int4* src = reinterpret_cast<const int4*>(smem + L::kItemOffset);
         const int4 a = src[0], b = src[1];
         it.s.q0 = __shfl_sync(0xffffffffu, a.x, 0), it.s.q_len = __shfl_sync(0xffffffffu, a.y, 0);
@@ -446,7 +453,7 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
         // that is at a long item would hold another that nobody else can take
         auto hand = [&]() {
             publish(it.t0);
-            const bool read = wait(item_empty, item_phase, DEV_TIMEOUT_EMPTY);
+            const bool read = wait_item(item_empty, item_phase, DEV_TIMEOUT_EMPTY);
             item_phase ^= 1u;
             return read;
         };
@@ -491,6 +498,7 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
                     for (int x = 0; x < D; x += 64)
                         tma_load_tile(base + L::kKvOffset + stage * L::kTileBytes + (x / 64) * L::kBoxBytes, map,
                                       kv_full(stage), x, it.kv, it.s.k0 + j * kAttnKeys);
+                    *progress = *progress + 1u;
                     if (++stage == ST) {
                         stage = 0;
                         phase ^= 1u;
@@ -658,7 +666,7 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
                 const int first = it.t0 + h * tile_tokens;
                 if (!ok || first >= it.s.q_len) continue;  // the tile has no rows
                 const int n = it.n[h];
-                ok = wait(stat_full(h), stat_phase[h], DEV_TIMEOUT_TMEM_FULL);
+                ok = wait_item(stat_full(h), stat_phase[h], DEV_TIMEOUT_TMEM_FULL);
                 stat_phase[h] ^= 1u;
                 if (!ok) continue;
                 if (n > 0) {

@@ -100,6 +100,31 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
     }
 }
 
+// The same for a wait that spans work of any length: the budget starts again whenever `progress` (shared memory, written by
+// another role at each bounded step) has changed since it last ran out.
+__device__ __forceinline__ bool mbar_wait_progress(uint32_t bar, uint32_t parity, volatile uint32_t* abort_flag,
+                                                   unsigned* status, unsigned code, volatile uint32_t* progress) {
+    if (mbar_try_wait(bar, parity)) return true;
+    long long t0 = clock64();
+    uint32_t seen = *progress;
+    for (uint32_t spin = 1;; ++spin) {
+        if (mbar_try_wait(bar, parity)) return true;
+        if ((spin & 63u) == 0u) {
+            if (*abort_flag) return false;
+            if (clock64() - t0 > *const_cast<volatile long long*>(&g_wait_budget_cycles)) {
+                const uint32_t now = *progress;
+                if (now == seen) {
+                    *abort_flag = 1u;
+                    atomicCAS(status, 0u, code);
+                    return false;
+                }
+                seen = now;
+                t0 = clock64();
+            }
+        }
+    }
+}
+
 // ---- TMA: 2-D tiled load global -> shared, completion on an mbarrier -------------
 __device__ __forceinline__ void tma_prefetch_desc(const void* tmap) {
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(tmap)) : "memory");

@@ -92,3 +92,23 @@ def test_i8gemm_launches_one_behind_the_other(cuda, M, N, K):
     assert bool(((outs[0].double() - want).abs() <= tol).all())
     assert all(cuda.equal(o, outs[0]) for o in outs)
     assert ops.device_status() == 0
+
+
+# ---- bounded waits -------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("q", [65, 200])
+def test_attention_waits_that_span_an_item_outlast_their_budget(cuda, q):
+    """Items of 2048 key tiles take about 3 ms; with a budget of 1 ms no wait may run out as long as its tiles go on.  One
+    row tile (the other's warps wait through the whole item) and two."""
+    from tacker_b200 import ops
+
+    keys = 1 << 18
+    a = Attention(cuda, [q], [keys], 1, 1, 128, "bf16", False, poison=False)
+    assert ops.device_status() == 0
+    ops.set_option("wait_budget_us", 1000)
+    try:
+        a.call()
+        cuda.cuda.synchronize()
+        assert ops.device_status() == 0
+    finally:
+        ops.set_option("wait_budget_us", 1000000)
+    a.check()
