@@ -440,7 +440,8 @@ typedef enum tk_type { TK_F32 = 0, TK_F16 = 1, TK_BF16 = 2 } tk_type;
  *   y may be x.  post = 1: a is normalised first, with post_gamma / post_beta [cols] (null = 1 / 0); pre is the
  *   norm of y (before y is rounded) that makes h, with pre_gamma / pre_beta.  layer 0: v / sqrt(mean v^2 + eps),
  *   1: (v - mean) / sqrt(var + eps).  gate (null = 1): fp32, rows r share gate row r / gate_rows (gate_rows >= rows: one
- *   row for all; 1: a row each; the tokens of a sequence each: a gate per sequence). */
+ *   row for all; 1: a row each; the tokens of a sequence each: a gate per sequence).  rows < 2^31, cols <= 2^30
+ *   (TK_ERR_SHAPE beyond). */
 int tk_norm_residual_rows(const void* a, int a_type, long long ld_a, int post, const float* post_gamma,
                           const float* post_beta, const float* gate, long long ld_gate, long long gate_rows, float scale,
                           const void* x, long long ld_x, void* y, long long ld_y, int x_type, const float* pre_gamma,
@@ -449,7 +450,8 @@ int tk_norm_residual_rows(const void* a, int a_type, long long ld_a, int post, c
 
 /* Rows to 8-bit integers: scales[r] = max |x[r]| / 127, codes[r][c] = x[r][c] / scales[r] rounded to the nearest
  * integer (the exact quotient with the fp32 scale; halves to even).  A row whose scale would be below 2^-126 gets scale 0
- * and codes 0; a row with a NaN or an infinity gets a scale that is one and codes 0. */
+ * and codes 0; a row with a NaN or an infinity gets a scale that is one and codes 0.  rows < 2^31, cols <= 2^30
+ * (TK_ERR_SHAPE beyond). */
 int tk_quantize_rows_i8(const void* x, int x_type, long long ld_x, void* codes, long long ld_codes, float* scales,
                         long long rows, int cols, void* stream);
 

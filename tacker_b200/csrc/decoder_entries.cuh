@@ -61,6 +61,7 @@ static int pow2_at_least(long long n, int lo, int hi) {
 }
 
 constexpr long long kMaxGridX = 0x7fffffffll;
+constexpr int kMaxCols = 1 << 30;  // of a row: column numbers and their steps of a block's threads stay in 32 bits
 
 // threads per row of the row kernels (sixteen columns each), threads and blocks of the launch
 struct RowShape {
@@ -290,7 +291,7 @@ TK_API int tk_norm_residual_rows(const void* a, int a_type, long long ld_a, int 
     if (rows == 0) return TK_OK;
     if (!a || (!y && !h) || ld_a < cols || (x && ld_x < cols) || (y && ld_y < cols) || (h && ld_h < cols)) return TK_ERR_ARGS;
     if (gate && (ld_gate < cols || gate_rows < 1)) return TK_ERR_ARGS;
-    if (rows > kMaxGridX) return TK_ERR_SHAPE;
+    if (rows > kMaxGridX || cols > kMaxCols) return TK_ERR_SHAPE;
     if (!aligned_to(a, type_bytes(a_type)) || !aligned_to(x, type_bytes(x_type)) || !aligned_to(y, type_bytes(x_type)) ||
         !aligned_to(h, type_bytes(h_type)))
         return TK_ERR_ALIGN;
@@ -335,7 +336,7 @@ TK_API int tk_quantize_rows_i8(const void* x, int x_type, long long ld_x, void* 
     if (rows < 0 || cols <= 0 || !type_ok(x_type)) return TK_ERR_ARGS;
     if (rows == 0) return TK_OK;
     if (!x || !codes || !scales || ld_x < cols || ld_codes < cols) return TK_ERR_ARGS;
-    if (rows > kMaxGridX) return TK_ERR_SHAPE;
+    if (rows > kMaxGridX || cols > kMaxCols) return TK_ERR_SHAPE;
     if (!aligned_to(x, type_bytes(x_type)) || !aligned_to(scales, 4)) return TK_ERR_ALIGN;
     int rc = on_this_device({x, codes, scales});
     if (rc != TK_OK) return rc;
