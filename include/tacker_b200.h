@@ -490,7 +490,7 @@ int tk_rope_qkv(const void* x, int x_type, long long ld_x, const float* bias, co
  * values rows k_start[i] .. k_start[i] + k_len[i] - 1 of k and v [kv_rows][kv_heads][dim].  Query head h reads key head
  * h / (heads / kv_heads).  causal: query t of q_len sees the keys j <= t + k_len - q_len.  A query that sees no key gives
  * zeros and lse -infinity.  out like q; lse [total_q][heads] = log sum exp of the scaled scores, or null.  type TK_F16 or
- * TK_BF16 for q, k, v and out; dim <= 256, total_q and kv_rows <= 2^30, total_q * heads < 2^31.  The three index arrays are device memory, read by the kernels (a captured
+ * TK_BF16 for q, k, v and out; dim <= 256, total_q and kv_rows <= 2^30, total_q * heads < 2^31 - 64.  The three index arrays are device memory, read by the kernels (a captured
  * graph replays with what they then hold); max_q and max_k, the longest q_len and k_len, choose the launch and may be
  * larger than the truth.  Keys and values outside the sequences' rows are never used, whatever they hold; inside them a
  * NaN or an infinity may reach every query of its sequence.

@@ -207,6 +207,9 @@ static int i8_split(long long tiles, int kblocks, int slots, int least) {
 }
 
 constexpr int kTokenRows = 64;  // most rows (tokens x heads of a group) of a sequence for the token form
+// query rows of a call: row numbers of the last block of rows, and of the block behind it that the token form's loop looks at,
+// stay in 32 bits
+constexpr long long kMaxTokenHeads = 0x7fffffffll - kTokenRows;
 
 template <int D, int TYPE>
 static int launch_attention_prompt(const AttnArgs& p, DeviceInfo* d, cudaStream_t st) {
@@ -482,7 +485,7 @@ TK_API int tk_attention_packed(const void* q, long long ld_q, const void* k, lon
         return TK_ERR_ARGS;
     if (heads % kv_heads) return TK_ERR_ARGS;
     if (n_seqs == 0 || total_q == 0) return TK_OK;
-    if (dim > 256 || static_cast<long long>(total_q) * heads > kMaxGridX || total_q > (1 << 30) || kv_rows > (1 << 30))
+    if (dim > 256 || static_cast<long long>(total_q) * heads > kMaxTokenHeads || total_q > (1 << 30) || kv_rows > (1 << 30))
         return TK_ERR_SHAPE;
     if (!q || !out || !q_start || !k_start || !k_len || (kv_rows > 0 && (!k || !v))) return TK_ERR_ARGS;
     if (ld_q < static_cast<long long>(heads) * dim || ld_out < static_cast<long long>(heads) * dim ||

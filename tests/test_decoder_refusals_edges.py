@@ -14,3 +14,13 @@ def test_rows_too_wide_for_32_bit_columns(ops, cols):  # noqa: F811
     wide = dict(ld_a=1 << 31, ld_x=1 << 31, ld_y=1 << 31, ld_h=1 << 31)
     refused(SHAPE, _call(ops.norm_residual_rows, {**NORM, **wide}), cols=cols)
     refused(SHAPE, ops.quantize_rows_i8, P, 0, 1 << 31, P, 1 << 31, P, 1, cols)
+
+
+def test_query_rows_whose_blocks_pass_32_bits(ops):  # noqa: F811
+    """The last block of 16 rows, and the four behind it, are numbered too: 2^31 - 65 tokens x heads is the most."""
+    good = dict(q=P, ld_q=64, k=P, ld_k=8, v=P, ld_v=8, out=P, ld_out=64, lse=P, type=1, q_start=P, k_start=P, k_len=P, n_seqs=1,
+                total_q=(1 << 28) - 8, kv_rows=100, max_q=1, max_k=50, heads=8, kv_heads=1, dim=8, scale=0.125, causal=1)
+    call = _call(ops.attention_packed, good)
+    for total_q in ((1 << 28) - 8, (1 << 28) - 1):
+        refused(SHAPE, call, total_q=total_q)
+    refused(SHAPE, call, total_q=(1 << 31) // 9, heads=9, ld_q=72, ld_out=72)
