@@ -436,8 +436,9 @@ int tk_tzgemm_batched(const void* A, const void* B, float* C, int M, int N, int 
 typedef enum tk_type { TK_F32 = 0, TK_F16 = 1, TK_BF16 = 2 } tk_type;
 
 /* y = x + scale * gate * post(a), h = pre(y): the residual stream between two blocks in one pass.
- *   a [rows][cols] of a_type; x, y of x_type; h of h_type.  x null: y = scale * gate * post(a); y or h null: not written;
- *   y may be x.  post = 1: a is normalised first, with post_gamma / post_beta [cols] (null = 1 / 0); pre is the
+ *   a [rows][cols] of a_type; x, y of x_type; h of h_type.  x null: y = scale * gate * post(a); y or h null: not written.
+ *   y and h may each be a or x in place, with the same element size and leading dimension, but not the same buffer
+ *   (TK_ERR_ARGS); other overlaps of outputs are not allowed.  post = 1: a is normalised first, with post_gamma / post_beta [cols] (null = 1 / 0); pre is the
  *   norm of y (before y is rounded) that makes h, with pre_gamma / pre_beta.  layer 0: v / sqrt(mean v^2 + eps),
  *   1: (v - mean) / sqrt(var + eps).  gate (null = 1): fp32, rows r share gate row r / gate_rows (gate_rows >= rows: one
  *   row for all; 1: a row each; the tokens of a sequence each: a gate per sequence).  rows < 2^31, cols <= 2^30

@@ -300,6 +300,17 @@ TK_API int tk_norm_residual_rows(const void* a, int a_type, long long ld_a, int 
         return TK_ERR_ALIGN;
     for (const float* f : {post_gamma, post_beta, gate, pre_gamma, pre_beta})
         if (!aligned_to(f, 4)) return TK_ERR_ALIGN;
+    // in place: each element is read and written by one thread, so the elements have to lie the same way
+    struct Rows {
+        const void* at;
+        long long ld;
+        int bytes;
+    };
+    const Rows in[2] = {{a, ld_a, type_bytes(a_type)}, {x, ld_x, type_bytes(x_type)}};
+    for (const Rows& o : {Rows{y, ld_y, type_bytes(x_type)}, Rows{h, ld_h, type_bytes(h_type)}})
+        for (const Rows& i : in)
+            if (o.at && o.at == i.at && (o.bytes != i.bytes || (rows > 1 && o.ld != i.ld))) return TK_ERR_ARGS;
+    if (y && y == h) return TK_ERR_ARGS;
     int rc = on_this_device({a, x, y, h, gate, post_gamma, post_beta, pre_gamma, pre_beta});
     if (rc != TK_OK) return rc;
     NormArgs p;

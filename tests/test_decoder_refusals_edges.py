@@ -24,3 +24,12 @@ def test_query_rows_whose_blocks_pass_32_bits(ops):  # noqa: F811
     for total_q in ((1 << 28) - 8, (1 << 28) - 1):
         refused(SHAPE, call, total_q=total_q)
     refused(SHAPE, call, total_q=(1 << 31) // 9, heads=9, ld_q=72, ld_out=72)
+
+
+def test_norm_in_place_needs_the_same_layout(ops):  # noqa: F811
+    """An output over an input whose elements or rows lie otherwise would overwrite what other threads still read; y and h
+    over each other have no result."""
+    call = _call(ops.norm_residual_rows, NORM)
+    for bad in (dict(y=2 * P, ld_y=72), dict(y=2 * P, ld_x=72), dict(y=P), dict(h=P), dict(y=P, a_type=1, ld_y=72), dict(h=2 * P, ld_h=72),
+                dict(h=2 * P, h_type=0), dict(h=P, h_type=0, ld_a=72), dict(h=3 * P), dict(h=3 * P, h_type=1)):
+        refused(ARGS, call, **bad)

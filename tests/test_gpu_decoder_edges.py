@@ -112,3 +112,30 @@ def test_attention_waits_that_span_an_item_outlast_their_budget(cuda, q):
     finally:
         ops.set_option("wait_budget_us", 1000000)
     a.check()
+
+
+# ---- the residual stream in place ----------------------------------------------------------------------------------
+@pytest.mark.parametrize("cols", [4096, 768, 59])
+@pytest.mark.parametrize("type", ["f32", "bf16"])
+@pytest.mark.parametrize("y_over,h_over", [("a", None), ("x", None), (None, "a"), (None, "x"), ("a", "x"), ("x", "a")])
+def test_norm_in_place(cuda, cols, type, y_over, h_over):
+    """y and h over a or x: what separate buffers get, bit for bit."""
+    from tacker_b200 import ops
+
+    rows, t, code = 700, ref.TYPES[type], ref.CODES[type]
+    g = cuda.Generator(device="cuda")
+    g.manual_seed(cols)
+    a, x = (cuda.randn(rows, cols, generator=g, device="cuda").to(t) for _ in "ax")
+    gamma = cuda.randn(cols, generator=g, device="cuda")
+
+    def call(a, x, y, h):
+        ops.norm_residual_rows(a.data_ptr(), code, cols, 1, gamma.data_ptr(), 0, 0, 0, 1, 0.5, x.data_ptr(), cols, y.data_ptr(), cols,
+                               code, gamma.data_ptr(), 0, h.data_ptr(), cols, code, 1, 1e-5, rows, cols)
+        cuda.cuda.synchronize()
+
+    y, h = cuda.zeros_like(a), cuda.zeros_like(a)
+    call(a, x, y, h)
+    here = {"a": a.clone(), "x": x.clone(), None: cuda.zeros_like(a)}
+    yy, hh = here[y_over], here[h_over]
+    call(here["a"], here["x"], yy, hh)
+    assert cuda.equal(yy, y) and cuda.equal(hh, h)
