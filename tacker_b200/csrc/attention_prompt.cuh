@@ -161,7 +161,7 @@ __device__ __forceinline__ float max_of(const uint32_t (&s)[32]) {
     }
     return max3(max3(m0, __uint_as_float(s[30]), __uint_as_float(s[31])), m1, m1);
 }
-// scores from `limit` on become -infinity; the limit as a mask of bits, which the compiler turns into predicates by sevens
+// scores from `limit` on become -infinity
 __device__ __forceinline__ void hide_from(uint32_t (&s)[32], int limit) {
     const uint32_t seen = limit >= 32 ? 0xffffffffu : limit <= 0 ? 0u : (1u << limit) - 1u;
 #pragma unroll

@@ -404,13 +404,11 @@ TK_API int tk_i8gemm(const void* A, long long lda, const float* scale_a, const v
     // Large products on CTA pairs: when their 256 x 256 tiles give half of the pairs of SMs something to do (64 tiles: 512 x 8192
     // x 4096 16.4 us, 19.0 in smaller tiles; 32 tiles: 300 x 4096 x 4096 15.4 us against 14.6)
     if ((M + 255ll) / 256 * ((N + 255ll) / 256) >= d->sm_count / 4) return launch_i8gemm_pair(A, lda, B, ldb, p, d, st);
-    // In between 128 x 128 tiles.  Joining ranges of k costs more than it gains once the tiles fill the device (300 x 4096 x
-    // 4096: 14.4 us unsplit, 15.1 with two ranges; 257 x 512 x 1024: 7.7 us, with eight 6.8).  A launch that has one CTA per
-    // SM at most takes the deeper ring.
+    // In between 128 x 128 tiles, fewer than the device has SMs (256 x 256 tiles that reach here are less than a quarter of
+    // that, each four of these), in a deep ring.  Joining ranges of k pays while the device is not full (257 x 512 x 1024:
+    // 7.7 us, with eight ranges 6.8) and costs more than it gains once it is (300 x 4096 x 4096: 14.4 us, 15.1 with two).
     const long long tiles = (M + 127ll) / 128 * tn;
-    const int split = i8_split(tiles, kblocks, d->sm_count, 1);
-    if (tiles * split <= d->sm_count) return launch_i8gemm<128, 6, false>(A, lda, B, ldb, p, split, st);
-    return launch_i8gemm<128, 3, false>(A, lda, B, ldb, p, split, st);
+    return launch_i8gemm<128, 6, false>(A, lda, B, ldb, p, i8_split(tiles, kblocks, d->sm_count, 1), st);
 }
 
 // pair i of a rotary head turns by pos * turns[i] full turns
@@ -513,7 +511,6 @@ TK_API int tk_attention_packed(const void* q, long long ld_q, const void* k, lon
     p.n_seqs = n_seqs, p.total_q = total_q, p.kv_rows = kv_rows, p.heads = heads, p.kv_heads = kv_heads, p.dim = dim;
     p.type = type, p.causal = causal, p.scale_log2 = scale * kLog2e;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    (void)workspace_bytes;
     const int group = heads / kv_heads;
     // what the tensor maps take: 16-byte rows of whole heads, a group within one tile, at least one key row
     const bool tiles = dim % 8 == 0 && dim <= 128 && group <= 128 && kv_rows > 0 && ld_q % 8 == 0 && ld_k % 8 == 0 &&

@@ -417,7 +417,7 @@ i8gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_cons
     volatile uint32_t* abort_flag = reinterpret_cast<volatile uint32_t*>(smem + L::kAbortOffset);
     const int pair = blockIdx.x >> 1, npairs = gridDim.x >> 1;
     const int tiles_m = (p.M + 255) / 256, tiles_n = (p.N + 255) / 256, kblocks = (p.K + kI8BK - 1) / kI8BK;
-    // at most 2^31 / 2^16 x 2^31 / 2^16 tiles: the launcher keeps the count below 2^31
+    // up to 2^22 tiles a side (M, N <= 2^30): the launcher keeps their product below 2^31
     const int tiles = tiles_m * tiles_n;
 
     if (warp == 0 && lane == 0) {
