@@ -5,7 +5,7 @@ import math
 import pytest
 
 import decoder_ref as ref
-from test_gpu_decoder import Attention, workspace
+from test_gpu_decoder import Attention, Block, at, normal, within, workspace
 
 pytestmark = pytest.mark.gpu
 
@@ -139,3 +139,212 @@ def test_norm_in_place(cuda, cols, type, y_over, h_over):
     yy, hh = here[y_over], here[h_over]
     call(here["a"], here["x"], yy, hh)
     assert cuda.equal(yy, y) and cuda.equal(hh, h)
+
+
+# ---- attention: precision of the forms -----------------------------------------------------------------------------
+def two_term_bound(a):
+    """(out, bound, out with weights rounded once) of calls with one token per sequence, in binary64.
+
+    Weights enter as p = hi + lo in the values' type: hi is off by half a step of p, lo by half a step of what hi left (or half
+    the smallest step there is), so that p is off by half_step^2.  What else is off is fp32: the scores (dim products, the scale,
+    the difference to the maximum, the power's 2 ulp) and the sums over n keys, once for the weights and once for the values."""
+    torch, U, f = a.torch, ref.U, torch_finfo(a)
+    outs, bounds, once = [], [], []
+    for i, n in enumerate(a.k_len):
+        q = a.q[i].double()
+        k, v = (z[a.k_start[i]:a.k_start[i] + n].double().repeat_interleave(a.heads // a.kv_heads, 1) for z in (a.k, a.v))
+        s = torch.einsum("hd,jhd->hj", q, k) * a.scale
+        size = (torch.einsum("hd,jhd->hj", q.abs(), k.abs()) * a.scale).amax(1)
+        m = s.amax(1, keepdim=True)
+        e = torch.exp(s - m)
+        total = e.sum(1, keepdim=True)
+        mix = lambda w, v: torch.einsum("hj,jhd->hd", w / total, v)  # noqa: E731, B023
+        out, spread = mix(e, v), mix(e, v.abs())
+        off = (a.dim + 4) * U * size + 4 * U * 1.45 * m[:, 0].abs() + 4 * U + n * U
+        outs.append(out)
+        bounds.append((ref.half_step(a.type) ** 2 + 2 * off[:, None]) * spread + ref.rounding(out, a.type) + n * f.tiny * f.eps / 2 * v.abs().amax())
+        once.append(mix(e.to(a.v.dtype).double(), v))
+    return (torch.stack(x) for x in (outs, bounds, once))
+
+
+def torch_finfo(a):
+    return a.torch.finfo(ref.TYPES[a.type])
+
+
+@pytest.mark.parametrize("type", ["f16", "bf16"])
+@pytest.mark.parametrize("dim,pad", [(64, 0), (128, 0), (64, 1)])
+@pytest.mark.parametrize("split", [True, False])
+def test_attention_tokens_do_not_round_their_weights(cuda, type, dim, pad, split):
+    """Values that nearly cancel show what rounding the weights once would cost: more than the bound.  (fp16 with heads of 128
+    is only checked against the bound: its fp32 part, (dim + 4) steps of the scores' size, is there larger than half a step of
+    fp16, which no test of the result can tell apart.)"""
+    k_len = [2, 3, 17, 40, 1024, 700]
+    a = Attention(cuda, [1] * len(k_len), k_len, 8, 2, dim, type, True, slab=1024, pad=pad, poison=False)
+    first = a.k[:1].clone()
+    a.k.mul_(0.05).add_(first)  # scores that are nearly equal
+    a.v.copy_(a.v.abs().add(1.0).mul(8))
+    a.v[1::2] = -a.v[0::2]
+    a.call(workspace(cuda) if split else None)
+    cuda.cuda.synchronize()
+    want, bound, once = two_term_bound(a)
+    got = a.out[:, :a.heads * dim].unflatten(1, (a.heads, dim))
+    within(cuda, got, want, bound, "out")
+    if type == "bf16" or dim == 64:
+        noticed = int(((once - want).abs() > bound).sum())
+        assert noticed > 0, "the bound would not notice weights that are rounded once"
+
+
+def test_calls_repeat_themselves_bit_for_bit(cuda):
+    """The same inputs again, after other kernels have used the shared memory: the same bits, in every form."""
+    ws = workspace(cuda)
+    calls = [Attention(cuda, [300, 1, 64], [300, 700, 900], 6, 2, 128, "bf16", True, slab=1000),
+             Attention(cuda, [1] * 5, [3, 700, 65, 900, 1], 8, 2, 64, "f16", True, slab=1000),
+             Attention(cuda, [70, 3], [70, 90], 4, 2, 40, "f16", True, pad=1, slab=100)]
+    for a in calls:
+        first = None
+        for i in range(6):
+            a.out.fill_(7)
+            a.call(ws)
+            got = a.out.clone(), a.lse.clone()
+            first = first or got
+            assert cuda.equal(got[0], first[0]) and cuda.equal(got[1], first[1])
+            x = cuda.full((512 * (i + 1), 512), math.nan if i % 2 else 100.0, dtype=cuda.float16, device="cuda")
+            x @ x[:512]
+            Attention(cuda, [130], [130], 7, 7, 128, "f16", False, seed=i).call(ws)
+
+
+@pytest.mark.parametrize("form", FORMS)
+def test_attention_scores_beyond_fp32(cuda, form):
+    """One key that scores +infinity for every other query (no number is left for it) and -infinity for the rest (which do
+    not notice it)."""
+    f = dict(FORMS[form])
+    q, dim, pad = f["q"], f["dim"], f.get("pad", 0)
+    a = Attention(cuda, [q], [200], 8, 2, dim, "bf16", False, pad=pad)
+    a.q.abs_().add_(0.1)
+    a.q[1::2] = -a.q[1::2]
+    a.k[150] = 3e38
+    for w in (workspace(cuda), None):
+        a.out.fill_(7)
+        a.call(w)
+        cuda.cuda.synchronize()
+        got = a.out[:, :8 * dim].unflatten(1, (8, dim))
+        assert bool(got[0::2].isnan().all()) and not bool(a.lse[0::2].isfinite().any())
+        rest = [i for i in range(200) if i != 150]
+        want, want_lse, tol, tol_lse = ref.attention(a.q, a.k[rest], a.v[rest], [0, q], [0], [199], a.scale, False, "bf16")
+        within(cuda, got[1::2], want[1::2], tol[1::2], "out")
+        within(cuda, a.lse[1::2], want_lse[1::2], tol_lse[1::2], "lse")
+
+
+@pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("form", FORMS)
+def test_attention_values_that_are_not_finite(cuda, form, value):
+    """A value that is not finite leaves no finite number in its element of the queries that see it, and touches nothing else:
+    not the other elements, not lse, not the other sequences."""
+    f = dict(FORMS[form])
+    q, dim, pad = f["q"], f["dim"], f.get("pad", 0)
+    a = Attention(cuda, [q, q], [200, 150], 8, 2, dim, "f16", False, pad=pad)
+    a.v[120, 1, 5] = value
+    a.call(workspace(cuda))
+    cuda.cuda.synchronize()
+    got = a.out[:, :8 * dim].unflatten(1, (8, dim)).clone()
+    assert not bool(got[:q, 4:, 5].isfinite().any())
+    a.v[120, 1, 5] = 0.0
+    want, want_lse, tol, tol_lse = ref.attention(a.q, a.k, a.v, a.q_start, a.k_start, a.k_len, a.scale, False, "f16")
+    got[:q, 4:, 5] = want[:q, 4:, 5].to(got.dtype)
+    within(cuda, got, want, tol, "out")
+    within(cuda, a.lse, want_lse, tol_lse, "lse")
+
+
+# ---- every combination of types ------------------------------------------------------------------------------------
+@pytest.mark.parametrize("a_type", ref.TYPES)
+@pytest.mark.parametrize("x_type", ref.TYPES)
+@pytest.mark.parametrize("h_type", ref.TYPES)
+@pytest.mark.parametrize("rows,cols", [(300, 4096), (37, 264)])
+def test_norm_types(cuda, a_type, x_type, h_type, rows, cols):
+    from tacker_b200 import ops
+
+    a, x = normal(cuda, 1, rows, cols, type=a_type, scale=3), normal(cuda, 2, rows, cols, type=x_type, scale=2)
+    g = [1 + normal(cuda, 3 + i, cols, scale=0.2) for i in range(4)]
+    y, h = (cuda.zeros(rows, cols, dtype=ref.TYPES[t], device="cuda") for t in (x_type, h_type))
+    ops.norm_residual_rows(at(a), ref.CODES[a_type], cols, 1, at(g[0]), at(g[1]), 0, 0, 1, 0.7, at(x), cols, at(y), cols, ref.CODES[x_type],
+                           at(g[2]), at(g[3]), at(h), cols, ref.CODES[h_type], 1, 1e-5, rows, cols)
+    cuda.cuda.synchronize()
+    wy, wh, ty, th = ref.norm(a, x, None, 1, 0.7, 1, *g, 1, 1e-5, x_type, h_type)
+    within(cuda, y, wy, ty, "y")
+    within(cuda, h, wh, th, "h")
+
+
+@pytest.mark.parametrize("x_type", ref.TYPES)
+@pytest.mark.parametrize("out_type", ref.TYPES)
+@pytest.mark.parametrize("dim,rot", [(128, 128), (72, 36)])
+def test_rope_types(cuda, x_type, out_type, dim, rot):
+    from tacker_b200 import ops
+
+    heads, kv_heads, tokens = 4, 2, 33
+    width = (heads + 2 * kv_heads) * dim
+    x, bias = normal(cuda, 1, tokens, width, type=x_type), normal(cuda, 2, width)
+    turns = cuda.tensor(ops.rope_turns(rot)[0], dtype=cuda.float64, device="cuda")
+    pos = cuda.arange(tokens, dtype=cuda.int32, device="cuda") * 1001
+    q, k, v = (cuda.zeros(tokens, h, dim, dtype=ref.TYPES[out_type], device="cuda") for h in (heads, kv_heads, kv_heads))
+    ops.rope_qkv(at(x), ref.CODES[x_type], width, at(bias), at(pos), at(turns), rot, 0, 1.1, tokens, heads, kv_heads, dim, at(q), heads * dim,
+                 at(k), kv_heads * dim, at(v), kv_heads * dim, ref.CODES[out_type])
+    cuda.cuda.synchronize()
+    want, tol = ref.rope(x, bias, pos, turns, rot, 0, 1.1, heads, kv_heads, dim, out_type)
+    within(cuda, cuda.cat((q, k, v), 1), want, tol, "heads")
+
+
+# ---- a block of them -----------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("q_len,past", [([100, 3, 37, 1], [0, 0, 0, 0]), ([1] * 9, [0, 5, 17, 63, 64, 200, 255, 100, 31])])
+def test_block_first_norm_and_its_rows_in_8_bits(cuda, q_len, past):
+    """The first norm's result, which the block's last norm overwrites, and its rounding to 8 bits."""
+    from tacker_b200 import ops
+
+    b = Block(cuda, q_len, past)
+    b.run()
+    h = cuda.zeros_like(b.h)
+    ops.norm_residual_rows(at(b.branch), 0, b.cols, 0, 0, 0, 0, 0, 1, 1.0, at(b.stream), b.cols, 0, 0, 0, at(b.gamma[0]), 0, at(h), b.cols, 2, 0,
+                           1e-6, b.T, b.cols)
+    cuda.cuda.synchronize()
+    _, want, _, tol = ref.norm(b.branch, b.stream, None, 1, 1.0, 0, None, None, b.gamma[0], None, 0, 1e-6, "f32", "bf16")
+    within(cuda, h, want, tol, "input of the projection")
+    codes, scales = ref.quantize(h)
+    assert cuda.equal(codes, b.c1.double()) and cuda.equal(scales, b.r1)
+
+
+def test_two_host_threads(cuda):
+    """Blocks of different shapes issued by two threads at once, each on a stream of its own: what each gives alone."""
+    import threading
+
+    blocks = [Block(cuda, [1] * 7, [3, 64, 200, 7, 0, 31, 90]), Block(cuda, [100, 3, 37, 80], [0, 20, 0, 5], dim=128)]
+    alone = []
+    for b in blocks:
+        b.run()
+        cuda.cuda.synchronize()
+        alone.append(b.outputs())
+    streams, errors, gate = [cuda.cuda.Stream() for _ in blocks], [], threading.Barrier(2)
+
+    def issue(b, s):
+        try:
+            gate.wait(30)
+            for _ in range(50):
+                b.run(s.cuda_stream)
+            s.synchronize()
+        except Exception as e:  # noqa: BLE001
+            errors.append(e)
+
+    threads = [threading.Thread(target=issue, args=x) for x in zip(blocks, streams)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(60)
+    assert not errors and not any(t.is_alive() for t in threads)
+    cuda.cuda.synchronize()
+    for b, want in zip(blocks, alone):
+        for x, y in zip(b.outputs(), want):
+            assert cuda.equal(x, y)
+
+
+def test_no_wait_ran_out(cuda):
+    from tacker_b200 import ops
+
+    assert ops.device_status() == 0
