@@ -16,8 +16,8 @@
 //
 // While the softmax of one tile runs, the tensor cores work for the other one.  P overwrites the columns of its S.
 // The running maximum is raised (and O multiplied by what that costs, in TMEM) only when the new one exceeds it by more
-// than 2^8: weights stay below 2^8, well inside the 16-bit types, the sums are fp32, and the final division makes it
-// exact; after the first tiles almost no item pays for a rescale.  P is rounded to the type of V because the tensor
+// than 2^8: weights stay below 2^8 (2^15 with the lift that fp16 gets), inside the 16-bit types, the sums are fp32, and the
+// final division makes it exact; after the first tiles almost no item pays for a rescale.  P is rounded to the type of V because the tensor
 // cores take two operands of one type; the row sum is taken before that rounding.
 //
 // Masks.  Keys beyond a row's limit get -infinity whatever their score is.  Weights of hidden keys are exact zeros, and
@@ -342,6 +342,7 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
                         unsigned* status) {
     using L = AttnSmem<D>;
     constexpr int ST = L::kStages;
+    constexpr float kUnlift = 1.0f / (1 << static_cast<int>(kPromptLift<TYPE>));
     constexpr uint32_t kO = 256;  // TMEM: S / P of tile 0 at column 0, of tile 1 at 128, O of the tiles at 256 and 384
     extern __shared__ __align__(1024) uint8_t attn_smem[];  // tiles need it; there is no room to align by hand
     uint8_t* smem = attn_smem;
@@ -676,7 +677,7 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
                     tc_fence_after_sync();
                 }
                 const float2 ml = *reinterpret_cast<const float2*>(smem + L::kStatOffset + (h * 128 + r) * 8);
-                const float inv = ml.y == 0.0f ? 0.0f : 1.0f / ml.y;
+                const float inv = ml.y == 0.0f ? 0.0f : kUnlift / ml.y;
                 // through shared memory, so that the bytes of a row are written by neighbouring lanes: a row per lane and
                 // store touches 32 lines with each instruction
                 const uint32_t t_o = tmem + (static_cast<uint32_t>(w32) << 16) + kO + h * 128;
@@ -795,7 +796,7 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
                     }
                 }
                 // a maximum of +infinity or NaN makes every weight of the row NaN, as the definition does
-                const float off = m == -INFINITY ? 0.0f : m == INFINITY ? NAN : -m * p.scale_log2;
+                const float off = m == -INFINITY ? 0.0f : m == INFINITY ? NAN : fmaf(-m, p.scale_log2, kPromptLift<TYPE>);
                 float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
                 {
                     uint32_t w[32];
@@ -828,7 +829,8 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
             if (!ok) break;
             o_phase ^= 1u;
             if (m == -INFINITY) l = 0.0f;  // every key of the row scored -infinity
-            *reinterpret_cast<float2*>(smem + L::kStatOffset + (h * 128 + r) * 8) = make_float2(m, l);
+            // the sum without the lift: the product takes the lift out of O
+            *reinterpret_cast<float2*>(smem + L::kStatOffset + (h * 128 + r) * 8) = make_float2(m, l * kUnlift);
             __syncwarp();
             if (lane == 0) mbar_arrive(stat_full(h));
         }

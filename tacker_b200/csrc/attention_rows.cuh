@@ -53,6 +53,14 @@ __device__ __forceinline__ int attn_seq_of(const AttnArgs& p, int row) {
 constexpr float kLn2 = 0.69314718055994530942f;
 constexpr float kLog2e = 1.44269504088896340736f;
 
+// Weights that enter a product in fp16 are lifted by a power of two, which the division by their sum takes out again: at 1 for
+// the largest weight, those below 2^-25 of it would be zeros, and 60000 keys of e^-17.5 each, 0.15 % of the sum, would be lost.
+// Prompts keep a maximum that may lag behind by 2^8, so that 2^15 is the largest weight there too.
+template <int TYPE>
+constexpr float kPromptLift = TYPE == kF16 ? 7.0f : 0.0f;  // powers of two
+template <int TYPE>
+constexpr float kTokenLift = TYPE == kF16 ? 32768.0f : 1.0f;
+
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

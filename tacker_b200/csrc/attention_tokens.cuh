@@ -215,7 +215,7 @@ attention_tokens_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
             for (int n = 0; n < 2; ++n)
 #pragma unroll
                 for (int w = 0; w < 2; ++w) {
-                    const float a0 = ex2(sc[n][2 * w] - off[w]), a1 = ex2(sc[n][2 * w + 1] - off[w]);
+                    const float a0 = ex2(sc[n][2 * w] - off[w]) * kTokenLift<TYPE>, a1 = ex2(sc[n][2 * w + 1] - off[w]) * kTokenLift<TYPE>;
                     l[w] += a0 + a1;
                     const uint32_t h = pack2(a0, a1, TYPE);
                     float h0, h1;
@@ -292,7 +292,7 @@ attention_tokens_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
             } else {
                 *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + row * p.ld_out + static_cast<long long>(hd) * p.dim + d) =
                     attn_result<TYPE>(v, sum);
-                if (d == 0 && p.lse) p.lse[row * p.heads + hd] = sum == 0.0f ? -INFINITY : (mm + log2f(sum)) * kLn2;
+                if (d == 0 && p.lse) p.lse[row * p.heads + hd] = sum == 0.0f ? -INFINITY : (mm + log2f(sum * (1.0f / kTokenLift<TYPE>))) * kLn2;
             }
         }
         if (rb + a.row_blocks < static_cast<int>((rows + kTokRows - 1) / kTokRows)) {
@@ -346,7 +346,7 @@ __global__ void attention_join_kernel(const AttnArgs p, const TokArgs a) {
     if (d < p.dim)
         *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + row * p.ld_out + static_cast<long long>(head) * p.dim + d) =
             attn_result<TYPE>(v, sum);
-    if (lane == 0 && p.lse) p.lse[item] = sum == 0.0f ? -INFINITY : (m + log2f(sum)) * kLn2;
+    if (lane == 0 && p.lse) p.lse[item] = sum == 0.0f ? -INFINITY : (m + log2f(sum * (1.0f / kTokenLift<TYPE>))) * kLn2;
 }
 
 }  // namespace tk

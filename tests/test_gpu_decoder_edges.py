@@ -194,6 +194,35 @@ def test_attention_tokens_do_not_round_their_weights(cuda, type, dim, pad, split
         assert noticed > 0, "the bound would not notice weights that are rounded once"
 
 
+@pytest.mark.parametrize("form", ["prompt", "tokens", "tokens, split", "rows"])
+@pytest.mark.parametrize("score", [-12.0, -17.5, -20.0])
+def test_attention_many_keys_of_little_weight(cuda, form, score):
+    """One key that takes almost all of the weight and 60000 that share the rest: weights of e^-12 to e^-20, the last two below
+    the steps of fp16, whose values decide the result.
+
+    Bound: as for scores and sums in fp32 everywhere; weights in fp16 half a step each, and at the end of its range half of its
+    smallest step, where the largest weight is 2^7 (prompts) or more."""
+    n, dim, q = 60001, 64, {"prompt": 70}.get(form, 1)
+    a = Attention(cuda, [q], [n], 1, 1, dim, "f16", False, pad=int(form == "rows"), scale=1.0, poison=False)
+    a.q.zero_()[:, :, 0] = 1.0
+    a.k.zero_()[1:, :, 0] = score
+    a.v[0] = 0
+    a.v[1:] = a.v[1:] * 100 + 1000
+    a.call(workspace(cuda) if form == "tokens, split" else None)
+    cuda.cuda.synchronize()
+    U, w = ref.U, math.exp(score)
+    total = 1 + (n - 1) * w
+    v = a.v[:, 0].double()
+    want = v[1:].sum(0) * w / total
+    spread = v[1:].abs().sum(0) * w / total
+    off = ((dim + 4) + 4 * 1.45) * U * abs(score) + 4 * U + n * U
+    bound = (ref.half_step("f16") + 2 * off) * spread + ref.rounding(want, "f16") + n * 2.0 ** -25 * 2.0 ** -7 * v.abs().max()
+    got = a.out[:, :dim].double()
+    within(cuda, got, want.expand_as(got), bound.expand_as(got), "out")
+    lse = cuda.full_like(a.lse.double(), math.log(total))
+    within(cuda, a.lse, lse, off + 4 * U * lse.abs(), "lse")
+
+
 def test_calls_repeat_themselves_bit_for_bit(cuda):
     """The same inputs again, after other kernels have used the shared memory: the same bits, in every form."""
     ws = workspace(cuda)
