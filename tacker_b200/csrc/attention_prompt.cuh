@@ -169,6 +169,11 @@ __device__ __forceinline__ void hide_from(uint32_t (&s)[32], int limit) {
         if (!(seen & (1u << i))) s[i] = 0xff800000u;
 }
 
+__device__ __forceinline__ void less(uint32_t (&s)[32], float x) {
+#pragma unroll
+    for (int i = 0; i < 32; ++i) s[i] = __float_as_uint(__uint_as_float(s[i]) - x);
+}
+
 // 32 weights 2^(scale s + off) of a row: their sums by fours and, rounded to the type, their pairs from w[at] on.  (A share
 // of the powers as polynomials on the multiply-add pipes, 1/8 to 3/8 of them, gained nothing: the tiles take turns on the
 // special-function units, and at full load the clock is set by the power limit.)
@@ -744,7 +749,8 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
             }
             const bool stored = token < tile_tokens && first + token < it.s.q_len;
             const int n = h ? it.n[1] : it.n[0];
-            float m = -INFINITY, l = 0.0f;
+            float m = -INFINITY, l = 0.0f, off = 0.0f, from = 0.0f;
+            bool any_far = false;
             for (int j = 0; j < n; ++j) {
                 ok = wait(s_full(h), s_phase, DEV_TIMEOUT_TMEM_FULL);
                 s_phase ^= 1u;
@@ -770,15 +776,17 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
                     tmem_ld_wait();
                     top = max3(top, max_of(s2), max_of(s3));
                 }
+                bool moved = j == 0;  // the maximum of some row of the warp
                 if (j == 0) {
                     m = top;
                 } else {
                     // a row's own scores decide, so that its result does not depend on its neighbours'; true from -infinity
-                    // and for NaN as well.  Rows that are not stored have no say: what lies there (of other sequences, behind
-                    // them, or in shared memory where no box reaches) may hold NaN, and would have its warp rescale for
-                    // every key tile (16384 keys, 65 tokens and NaN behind them: 233 us instead of 206)
+                    // and for NaN as well.  Rows that are not stored have no say: what lies there (of other sequences,
+                    // behind them, or in shared memory where no box reaches) may hold NaN, and would have its warp rescale
+                    // for every key tile (16384 keys, 65 tokens and NaN behind them: 233 us instead of 206)
                     const bool raise = stored && !((top - m) * p.scale_log2 <= 8.0f);
-                    if (__any_sync(0xffffffffu, raise)) {
+                    moved = __any_sync(0xffffffffu, raise);
+                    if (moved) {
                         // the scores of this tile follow the product that last added to O: O is at rest
                         const float up = raise ? max2(m, top) : m;
                         const float keep = !raise ? 1.0f : m == -INFINITY ? 0.0f : ex2((m - up) * p.scale_log2);
@@ -795,8 +803,17 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
                         }
                     }
                 }
-                // a maximum of +infinity or NaN makes every weight of the row NaN, as the definition does
-                const float off = m == -INFINITY ? 0.0f : m == INFINITY ? NAN : fmaf(-m, p.scale_log2, kPromptLift<TYPE>);
+                if (moved) {
+                    // a maximum of +infinity or NaN makes every weight of the row NaN, as the definition does
+                    off = m == -INFINITY ? 0.0f : m == INFINITY ? NAN : fmaf(-m, p.scale_log2, kPromptLift<TYPE>);
+                    // scale s + off rounds off to its last place: from scores of 2^16 on, where that is more than 2^-8, the
+                    // maximum is taken from the scores first, which is exact near it
+                    const bool far = stored && fabsf(off) > 65536.0f;
+                    from = far ? m : 0.0f;
+                    if (far) off = kPromptLift<TYPE>;
+                    any_far = __any_sync(0xffffffffu, far);
+                }
+                if (any_far) less(s0, from), less(s1, from), less(s2, from), less(s3, from);
                 float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
                 {
                     uint32_t w[32];

@@ -223,6 +223,38 @@ def test_attention_many_keys_of_little_weight(cuda, form, score):
     within(cuda, a.lse, lse, off + 4 * U * lse.abs(), "lse")
 
 
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("type,q0,k0", [("bf16", 1.0, 2.0 ** 17), ("bf16", 1.0, 3e7), ("bf16", -1.0, 1e9), ("bf16", 3.0, 1e20), ("bf16", 1.0, 3e37),
+                                        ("f16", 1.0, 60000.0), ("f16", 55.0, 60000.0), ("f16", -60000.0, 60000.0)])
+def test_attention_scores_of_any_size(cuda, form, type, q0, k0):
+    """Two keys whose scores are larger than all others by far, in two different key tiles: each weighs one half, whatever
+    their size; and the same with all scores negative."""
+    f = dict(FORMS[form])
+    q, dim, pad = f["q"], f["dim"], f.get("pad", 0)
+    a = Attention(cuda, [q], [200], 8, 2, dim, type, False, pad=pad, scale=1.0)
+    for lowest in (False, True):
+        a.q.zero_()[:, :, 0] = q0
+        a.k.zero_()
+        if lowest:  # the others lie further from zero
+            a.k[:, :, 0] = -math.copysign(k0, q0)
+            a.k[7, :, 0] = a.k[150, :, 0] = -math.copysign(k0 / 2, q0)
+        else:
+            a.k[7, :, 0] = a.k[150, :, 0] = math.copysign(k0, q0)
+        a.call(workspace(cuda))
+        cuda.cuda.synchronize()
+        score = a.q[0, 0, 0].double() * a.k[7, 0, 0].double()
+        v = a.v.double().repeat_interleave(4, 1)
+        want = ((v[7] + v[150]) / 2).expand(q, 8, dim)
+        # weights are powers 2^(scale s + off) with off rounded to 32 bits: equal for equal scores, but no powers of two, and
+        # prompts round them once to the type (half a step each, on both values; the sum is taken before)
+        spread = (v[7].abs() + v[150].abs()) / 2
+        bound = (8 * ref.U + ref.half_step(type) * (form == "prompt")) * spread + ref.rounding(want, type)
+        got = a.out[:, :8 * dim].unflatten(1, (8, dim))
+        within(cuda, got, want, bound, "out")
+        lse = (score + math.log(2)).expand(q, 8)
+        within(cuda, a.lse, lse, 8 * ref.U * lse.abs(), "lse")
+
+
 def test_calls_repeat_themselves_bit_for_bit(cuda):
     """The same inputs again, after other kernels have used the shared memory: the same bits, in every form."""
     ws = workspace(cuda)
