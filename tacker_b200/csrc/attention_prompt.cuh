@@ -749,8 +749,8 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
             }
             const bool stored = token < tile_tokens && first + token < it.s.q_len;
             const int n = h ? it.n[1] : it.n[0];
-            float m = -INFINITY, l = 0.0f, off = 0.0f, from = 0.0f;
-            bool any_far = false;
+            float m = -INFINITY, l = 0.0f, off = 0.0f;
+            bool far = false;
             for (int j = 0; j < n; ++j) {
                 ok = wait(s_full(h), s_phase, DEV_TIMEOUT_TMEM_FULL);
                 s_phase ^= 1u;
@@ -776,15 +776,17 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
                     tmem_ld_wait();
                     top = max3(top, max_of(s2), max_of(s3));
                 }
-                bool moved = j == 0;  // the maximum of some row of the warp
+                bool moved = true;  // the maximum of some row of the warp
                 if (j == 0) {
                     m = top;
                 } else {
                     // a row's own scores decide, so that its result does not depend on its neighbours'; true from -infinity
                     // and for NaN as well.  Rows that are not stored have no say: what lies there (of other sequences,
                     // behind them, or in shared memory where no box reaches) may hold NaN, and would have its warp rescale
-                    // for every key tile (16384 keys, 65 tokens and NaN behind them: 233 us instead of 206)
-                    const bool raise = stored && !((top - m) * p.scale_log2 <= 8.0f);
+                    // for every key tile (16384 keys, 65 tokens and NaN behind them: 233 us instead of 206).  Rows with scores
+                    // so far from zero that they need what follows below come here for every tile, so that others do not
+                    // pass by it
+                    const bool raise = stored && (far || !((top - m) * p.scale_log2 <= 8.0f));
                     moved = __any_sync(0xffffffffu, raise);
                     if (moved) {
                         // the scores of this tile follow the product that last added to O: O is at rest
@@ -808,12 +810,13 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
                     off = m == -INFINITY ? 0.0f : m == INFINITY ? NAN : fmaf(-m, p.scale_log2, kPromptLift<TYPE>);
                     // scale s + off rounds off to its last place: from scores of 2^16 on, where that is more than 2^-8, the
                     // maximum is taken from the scores first, which is exact near it
-                    const bool far = stored && fabsf(off) > 65536.0f;
-                    from = far ? m : 0.0f;
-                    if (far) off = kPromptLift<TYPE>;
-                    any_far = __any_sync(0xffffffffu, far);
+                    far = stored && fabsf(off) > 65536.0f;
+                    if (__any_sync(0xffffffffu, far)) {
+                        const float from = far ? m : 0.0f;
+                        less(s0, from), less(s1, from), less(s2, from), less(s3, from);
+                        if (far) off = kPromptLift<TYPE>;
+                    }
                 }
-                if (any_far) less(s0, from), less(s1, from), less(s2, from), less(s3, from);
                 float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
                 {
                     uint32_t w[32];

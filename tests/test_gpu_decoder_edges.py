@@ -255,6 +255,38 @@ def test_attention_scores_of_any_size(cuda, form, type, q0, k0):
         within(cuda, a.lse, lse, 8 * ref.U * lse.abs(), "lse")
 
 
+@pytest.mark.parametrize("type", ["f16", "bf16"])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_attention_large_scores_in_some_rows(cuda, type, dim):
+    """Rows with scores of ordinary size, of hundreds of thousands and in between side by side in every warp, over several
+    key tiles, causal: each by its own rule.
+
+    Scores of size B are exact to B * 2^-24 times the additions, so that a row's weights are off by that: with one element per
+    head that is not zero, the score is one product and its scale, exact but for one rounding each."""
+    q = 300
+    a = Attention(cuda, [q], [700], 4, 2, dim, type, True, scale=1.0)
+    size = 4.0 ** (cuda.arange(q, device="cuda") % 10)  # 1 .. 262144
+    a.q.zero_()[:, :, 0] = cuda.where(size > 60000, 1.0, size).to(a.q.dtype)[:, None]
+    a.q[:, :, 1] = cuda.where(size > 60000, 32768.0, 0.0).to(a.q.dtype)[:, None]
+    k = cuda.randn(700, 2, generator=cuda.Generator(device="cuda").manual_seed(3), device="cuda")
+    a.k.zero_()[:, :, 0] = k.to(a.k.dtype)
+    a.k[:, :, 1] = (k * 8).round().to(a.k.dtype)
+    a.call(workspace(cuda))
+    cuda.cuda.synchronize()
+    want, want_lse, _, _ = ref.attention(a.q, a.k, a.v, a.q_start, a.k_start, a.k_len, 1.0, True, type)
+    s = cuda.einsum("thd,jhd->htj", a.q.double(), a.k.double().repeat_interleave(2, 1))
+    see = cuda.arange(700, device="cuda")[None] <= cuda.arange(q, device="cuda")[:, None] + 400
+    big = s.masked_fill(~see, 0).abs().amax(2).t()
+    p = cuda.softmax(s.masked_fill(~see, -math.inf), 2)
+    spread = cuda.einsum("htj,jhd->thd", p, a.v.double().abs().repeat_interleave(2, 1))
+    # score: two products' sum (2 U), times log2 e and the rounded maximum (2 U), the difference and the power (4 U); n sums
+    off = (4 * 1.45 * big + 4 + 700) * ref.U
+    bound = (ref.half_step(type) + 2 * off[..., None]) * spread + ref.rounding(want, type) + 700 * 2.0 ** -25 * (type == "f16") * 4.5 * 2.0 ** -7
+    got = a.out[:, :4 * dim].unflatten(1, (4, dim))
+    within(cuda, got, want, bound, "out")
+    within(cuda, a.lse, want_lse, off + 4 * ref.U * want_lse.abs(), "lse")
+
+
 def test_calls_repeat_themselves_bit_for_bit(cuda):
     """The same inputs again, after other kernels have used the shared memory: the same bits, in every form."""
     ws = workspace(cuda)
