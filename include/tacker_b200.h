@@ -431,18 +431,19 @@ int tk_tzgemm_batched(const void* A, const void* B, float* C, int M, int N, int 
  * all buffers are device memory of the current device (a buffer of another one is refused with TK_ERR_ARGS), rows are
  * `ld` elements apart, and everything works in a captured graph.  Calls with nothing to do (0 rows, tokens or
  * sequences) return TK_OK.  Statistics, sums and scores are held in fp32 (8-bit products in 32-bit integers); a result
- * is rounded once to its type.  Wide accesses need 16-byte aligned buffers and leading dimensions that are multiples of
- * 8; other alignments take slower forms of the same operators where no refusal is stated. */
+ * is rounded once to its type (attention of prompts also rounds its weights, see there).  Wide accesses need 16-byte
+ * aligned buffers and leading dimensions that are multiples of 8; other alignments take slower forms of the same
+ * operators where no refusal is stated. */
 typedef enum tk_type { TK_F32 = 0, TK_F16 = 1, TK_BF16 = 2 } tk_type;
 
 /* y = x + scale * gate * post(a), h = pre(y): the residual stream between two blocks in one pass.
  *   a [rows][cols] of a_type; x, y of x_type; h of h_type.  x null: y = scale * gate * post(a); y or h null: not written.
  *   y and h may each be a or x in place, with the same element size and leading dimension, but not the same buffer
- *   (TK_ERR_ARGS); other overlaps of outputs are not allowed.  post = 1: a is normalised first, with post_gamma / post_beta [cols] (null = 1 / 0); pre is the
- *   norm of y (before y is rounded) that makes h, with pre_gamma / pre_beta.  layer 0: v / sqrt(mean v^2 + eps),
- *   1: (v - mean) / sqrt(var + eps).  gate (null = 1): fp32, rows r share gate row r / gate_rows (gate_rows >= rows: one
- *   row for all; 1: a row each; the tokens of a sequence each: a gate per sequence).  rows < 2^31, cols <= 2^30
- *   (TK_ERR_SHAPE beyond). */
+ *   (TK_ERR_ARGS); other overlaps of outputs are not allowed.  post = 1: a is normalised first, with post_gamma /
+ *   post_beta [cols] (null = 1 / 0); pre is the norm of y (before y is rounded) that makes h, with pre_gamma / pre_beta.
+ *   layer 0: v / sqrt(mean v^2 + eps), 1: (v - mean) / sqrt(var + eps).  gate (null = 1): fp32, rows r share gate row
+ *   r / gate_rows (gate_rows >= rows: one row for all; 1: a row each; the tokens of a sequence each: a gate per
+ *   sequence).  rows < 2^31, cols <= 2^30 (TK_ERR_SHAPE beyond). */
 int tk_norm_residual_rows(const void* a, int a_type, long long ld_a, int post, const float* post_gamma,
                           const float* post_beta, const float* gate, long long ld_gate, long long gate_rows, float scale,
                           const void* x, long long ld_x, void* y, long long ld_y, int x_type, const float* pre_gamma,
@@ -451,15 +452,15 @@ int tk_norm_residual_rows(const void* a, int a_type, long long ld_a, int post, c
 
 /* Rows to 8-bit integers: scales[r] = max |x[r]| / 127, codes[r][c] = x[r][c] / scales[r] rounded to the nearest
  * integer (the exact quotient with the fp32 scale; halves to even).  A row whose scale would be below 2^-126 gets scale 0
- * and codes 0; a row with a NaN or an infinity gets a scale that is one and codes 0.  rows < 2^31, cols <= 2^30
- * (TK_ERR_SHAPE beyond). */
+ * and codes 0.  A row with a NaN or an infinity gets that NaN or infinity (not 1.0) as its scale, and codes 0, so that
+ * products with it are NaN.  rows < 2^31, cols <= 2^30 (TK_ERR_SHAPE beyond). */
 int tk_quantize_rows_i8(const void* x, int x_type, long long ld_x, void* codes, long long ld_codes, float* scales,
                         long long rows, int cols, void* stream);
 
 /* out[m][n] = (sum_k A[m][k] B[n][k]) * scale_a[m] * scale_b[n] + bias[n]: 8-bit signed integers A [M][K] (tokens) and
  * B [N][K] (output channels), exact 32-bit sums, fp32 scales [M] and [N], fp32 bias [N] or null, out [M][N] of out_type.
- * Any M, N <= 2^30 and K <= 131071 (TK_ERR_SHAPE beyond: the sums would overflow); A and B 16-byte aligned, lda and ldb multiples
- * of 16 (TK_ERR_ALIGN). */
+ * Any M, N <= 2^30 and K <= 131071 (TK_ERR_SHAPE beyond: the sums would overflow); A and B 16-byte aligned, lda and ldb
+ * multiples of 16 (TK_ERR_ALIGN). */
 int tk_i8gemm(const void* A, long long lda, const float* scale_a, const void* B, long long ldb, const float* scale_b,
               const float* bias, void* out, long long ld_out, int out_type, int M, int N, int K, void* stream);
 
@@ -491,12 +492,18 @@ int tk_rope_qkv(const void* x, int x_type, long long ld_x, const float* bias, co
  * values rows k_start[i] .. k_start[i] + k_len[i] - 1 of k and v [kv_rows][kv_heads][dim].  Query head h reads key head
  * h / (heads / kv_heads).  causal: query t of q_len sees the keys j <= t + k_len - q_len.  A query that sees no key gives
  * zeros and lse -infinity.  out like q; lse [total_q][heads] = log sum exp of the scaled scores, or null.  type TK_F16 or
- * TK_BF16 for q, k, v and out; dim <= 256, total_q and kv_rows <= 2^30, total_q * heads < 2^31 - 64.  The three index arrays are device memory, read by the kernels (a captured
- * graph replays with what they then hold); max_q and max_k, the longest q_len and k_len, choose the launch and may be
- * larger than the truth.  Keys and values outside the sequences' rows are never used, whatever they hold; inside them a
- * NaN or an infinity may reach every query of its sequence.
- * workspace: device memory, 16-byte aligned, not shared by calls that may overlap; scratch for work split over long key
- * axes.  A call splits as far as it has room; null or 0 bytes = no split.
+ * TK_BF16 for q, k, v and out; dim <= 256, total_q and kv_rows <= 2^30, total_q * heads < 2^31 - 64.  The three index
+ * arrays are device memory, read by the kernels (a captured graph replays with what they then hold); max_q and max_k,
+ * the longest q_len and k_len, choose the form of the launch and may be larger than the truth.
+ * Forms: up to 64 rows per sequence (max_q * heads / kv_heads) are tokens, which hold their weights as two terms of the
+ * type; more are prompts, which round each weight once to the type (at most half a step of it on every value); head
+ * sizes above 128 or not multiples of 8, groups above 128, unaligned rows and scales that are not positive take a form of
+ * one warp per query row and head, with weights in fp32, whose time is far from that of the others.  Results of
+ * different forms differ by that rounding; the same call repeats itself bit for bit.
+ * Keys and values outside the sequences' rows are never used, whatever they hold; inside them a NaN or an infinity may
+ * reach every query of its sequence that sees a key (what it reaches is NaN or infinite).
+ * workspace: device memory, 16-byte aligned, not shared by calls that may overlap; scratch for the work of tokens, whose
+ * long key axes are split as far as it has room (null or 0 bytes = no split).  Prompts do not split their keys.
  * TK_ATTENTION_WORKSPACE bytes are enough for every split that pays. */
 #define TK_ATTENTION_WORKSPACE (64u << 20)
 int tk_attention_packed(const void* q, long long ld_q, const void* k, long long ld_k, const void* v, long long ld_v,
@@ -513,9 +520,9 @@ int tk_attention_packed(const void* q, long long ld_q, const void* k, long long 
  *   super-tile width bn writes for [start, end); work[c] (optional) += super-tiles of CTA c.
  * tk_plan_stencil: planes[b*nz + k] += 1 for every plane k of bundle b some warp computes, loads[b*nz + k]
  *   (optional) += 1 for every plane streamed; split = {slabs per bundle, planes per slab} chosen for the launch.
- * tk_plan_attention: cover[kv * sum(q_len) + token] += 1 for every token and key head that a launch of `blocks` blocks of
- *   the attention kernel for prompts works on (tile_tokens = 128 / group); CTA c of `ctas` starts as block order[c] and takes
- *   over blocks order[c + ctas], order[c + 2 ctas] ... */
+ * tk_plan_attention: cover[kv * sum(q_len) + token] += 1 for every token and key head that a launch of `blocks` blocks
+ *   of the attention kernel for prompts works on (tile_tokens = 128 / group); CTA c of `ctas` starts as block order[c]
+ *   and takes over blocks order[c + ctas], order[c + 2 ctas] ... */
 int tk_plan_tzgemm(int M, int N, int bn, int start, int end, int ctas, int* cover, int* work);
 int tk_plan_tzgemm_m256(int M, int N, int start, int end, int ctas, int* cover); /* 256 x 256 super-tile kernel */
 int tk_plan_stencil(int nz, int blocks_start, int blocks_end, int gx, int gy, int ctas, int warps_per_cta,

@@ -17,17 +17,18 @@
 // While the softmax of one tile runs, the tensor cores work for the other one.  P overwrites the columns of its S.
 // The running maximum is raised (and O multiplied by what that costs, in TMEM) only when the new one exceeds it by more
 // than 2^8: weights stay below 2^8 (2^15 with the lift that fp16 gets), inside the 16-bit types, the sums are fp32, and the
-// final division makes it exact; after the first tiles almost no item pays for a rescale.  P is rounded to the type of V because the tensor
-// cores take two operands of one type; the row sum is taken before that rounding.
+// final division makes it exact; after the first tiles almost no item pays for a rescale.  P is rounded to the type of V
+// because the tensor cores take two operands of one type: half a step on each value, error against binary64 1.2 to 1.3
+// times that of rounding the result alone.  The row sum is taken before that rounding.
 //
 // Masks.  Keys beyond a row's limit get -infinity whatever their score is.  Weights of hidden keys are exact zeros, and
 // the values behind the sequence's last key within the last 16 that an MMA reads are zeroed in shared memory, so that
 // nothing they hold (NaN included) can enter.
 //
 // Bound: per key tile and SM the two tiles take 2 x 2 x 512 cycles of the tensor pipe (head size 128) and 32768 powers of
-// two = 2048 cycles of the special-function units, both at the same time; measured are 3050 cycles, 1930 of them the softmax
+// two = 2048 cycles of the special-function units, both at the same time; measured are about 3100 cycles, 1930 of them the softmax
 // of a tile (scores from tensor memory and their maximum 370, powers 1460) and 1000 from its weights to its next scores.
-// 8192 tokens x 16 heads x 128, causal: 220 us = 1250 TFLOP/s of visible products.
+// 8192 tokens x 16 heads x 128, causal: 231 us = 1190 TFLOP/s of visible products; sixteen packed prompts 91 us.
 #pragma once
 #include <cuda.h>
 
