@@ -279,10 +279,12 @@ __host__ __device__ __forceinline__ long long attn_items_of(int q_len, int kv_he
 struct AttnWindow {
     const AttnArgs& p;
     const int tile_tokens, lane;
+    uint32_t* progress;
     AttnSeq s;
     long long mine, upto;  // items of this lane's sequence, and of the window up to and with it
 
     __device__ __forceinline__ void load(int base) {
+        if (lane == 0) atomicAdd(progress, 1u);
         s.q_len = 0, s.q0 = 0, s.k0 = 0, s.k_len = 0;
         if (base + lane < p.n_seqs) s.load(p, base + lane);
         mine = attn_items_of(s.q_len, p.kv_heads, tile_tokens);
@@ -369,7 +371,8 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
     const uint32_t item_full = bars + 8u * (2 * ST + 16), item_empty = item_full + 8, claim_bar = item_full + 16;
     volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + L::kTmemSlotOffset);
     volatile uint32_t* abort_flag = reinterpret_cast<volatile uint32_t*>(smem + L::kAbortOffset);
-    volatile uint32_t* progress = reinterpret_cast<volatile uint32_t*>(smem + L::kProgressOffset);  // tiles asked for
+    // steps of the producer (tiles asked for) and of the search for items (blocks taken over, windows looked through)
+    uint32_t* progress = reinterpret_cast<uint32_t*>(smem + L::kProgressOffset);
 
     if (warp == 12) {
         if (lane == 0) {
@@ -413,7 +416,7 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
     auto wait = [&](uint32_t bar, uint32_t parity, unsigned code) {
         return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, status, code)) != 0;
     };
-    // a wait that spans an item, whose length has no bound: the producer's steps keep it alive
+    // a wait that spans an item or the search for the next one, which have no bound: their steps keep it alive
     auto wait_item = [&](uint32_t bar, uint32_t parity, unsigned code) {
         return __all_sync(0xffffffffu, mbar_wait_progress(bar, parity, abort_flag, status, code, progress)) != 0;
     };
@@ -438,7 +441,7 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
       fewer_registers<kAttnOtherRegs>();
       if (warp == 14) {
         // ---------------- items ----------------
-        AttnWindow window = {p, tile_tokens, lane};
+        AttnWindow window = {p, tile_tokens, lane, progress};
         window.load(0);
         AttnSeek seek;
         uint32_t claim_phase = 0;
@@ -466,6 +469,7 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
         };
         auto take = [&](int& index) {
             if (lane == 0) {
+                atomicAdd(progress, 1u);
                 fence_proxy_async_smem();  // the last result has been read
                 mbar_arrive_expect_tx(claim_bar, 16);
                 claim_request(base + L::kClaimOffset, claim_bar);
@@ -505,7 +509,7 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
                     for (int x = 0; x < D; x += 64)
                         tma_load_tile(base + L::kKvOffset + stage * L::kTileBytes + (x / 64) * L::kBoxBytes, map,
                                       kv_full(stage), x, it.kv, it.s.k0 + j * kAttnKeys);
-                    *progress = *progress + 1u;
+                    atomicAdd(progress, 1u);
                     if (++stage == ST) {
                         stage = 0;
                         phase ^= 1u;

@@ -114,6 +114,30 @@ def test_attention_waits_that_span_an_item_outlast_their_budget(cuda, q):
     a.check()
 
 
+def test_attention_search_for_items_outlasts_the_budget(cuda):
+    """Two sequences with tokens among 600000 without: the search for their items, and the blocks that have none, take several
+    times the budget of a wait, and no wait runs out."""
+    from tacker_b200 import ops
+
+    n, kv_heads, dim = 600_000, 8, 64
+    a = Attention(cuda, [200, 130], [200, 130], 8, kv_heads, dim, "f16", True)
+    many = [cuda.zeros(n + 1, dtype=cuda.int32, device="cuda") for _ in range(3)]
+    many[0][1000:] = 200
+    many[0][n:] = 330  # sequence 999 has 200 tokens, the last one 130
+    many[1][n - 1] = 200
+    many[2][999], many[2][n - 1] = 200, 130
+    assert ops.device_status() == 0
+    ops.set_option("wait_budget_us", 1000)
+    try:
+        ops.attention_packed(at(a.q), 8 * dim, at(a.k), 8 * dim, at(a.v), 8 * dim, at(a.out), 8 * dim, at(a.lse), 1, *(at(x) for x in many), n,
+                             a.total, a.rows, 200, 200, 8, 8, dim, a.scale, 1)
+        cuda.cuda.synchronize()
+        assert ops.device_status() == 0
+    finally:
+        ops.set_option("wait_budget_us", 1000000)
+    a.check()
+
+
 # ---- the residual stream in place ----------------------------------------------------------------------------------
 @pytest.mark.parametrize("cols", [4096, 768, 59])
 @pytest.mark.parametrize("type", ["f32", "bf16"])
